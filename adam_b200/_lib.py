@@ -33,6 +33,11 @@ class DecoderDesc(ctypes.Structure):
                 ("tp_rank", u32), ("tp_size", u32), ("flags", u32)]
 
 
+class KvDesc(ctypes.Structure):
+    """``adam_b200_kv_desc`` of include/adam_b200.h."""
+    _fields_ = [(n, u32) for n in ("n_layer", "n_head_kv", "head_dim", "kv_dtype", "page_size", "n_pages", "max_seqs", "max_pages")]
+
+
 # name -> (restype, argtypes); the part-1 entries follow adamah.c's signatures
 _SIGS = {
     "adamah_init": (c_int, []),
@@ -136,6 +141,18 @@ _SIGS = {
     "adam_b200_ar_open": (c_int, [u32, c_void_p]),
     "adam_b200_ar_allreduce": (c_int, [u32, u64, u32]),
     "adam_b200_ar_destroy": (c_int, [u32]),
+    "adam_b200_map_ptr": (c_int, [u32, POINTER(u64), POINTER(u64)]),
+    "adam_b200_kv_create": (c_int, [POINTER(KvDesc), POINTER(u32)]),
+    "adam_b200_kv_destroy": (c_int, [u32]),
+    "adam_b200_kv_extend": (c_int, [u32, u32, c_void_p, c_void_p]),
+    "adam_b200_kv_fork": (c_int, [u32, u32, u32, c_void_p, u32]),
+    "adam_b200_kv_truncate": (c_int, [u32, u32, c_void_p, c_void_p]),
+    "adam_b200_kv_compact": (c_int, [u32, POINTER(u32)]),
+    "adam_b200_kv_state": (c_int, [u32, POINTER(u32), c_void_p, c_void_p]),
+    "adam_b200_kv_ptr": (c_int, [u32, u32, POINTER(u64), POINTER(u64)]),
+    "map_qk_norm_rope_kv_dev": (c_int, [u32] * 15 + [f32, f32]),
+    "map_attn_kv_dev": (c_int, [u32] * 12 + [f32, f32]),
+    "map_sample_dev": (c_int, [u32] * 7),
     "adam_b200_noalloc_prepare": (c_int, []),
     "adam_b200_ar_set_wait_us": (c_int, [u32, u64]),
     "adam_b200_ar_reset": (c_int, [u32]),

@@ -14,7 +14,7 @@ from typing import Dict, Optional
 import numpy as np
 
 from . import _lib
-from ._lib import DecodePlanOp  # noqa: F401  (re-exported)
+from ._lib import DecodePlanOp, KvDesc  # noqa: F401  (re-exported)
 from . import constants as C
 from .host_arrays import HostArrays
 
@@ -26,6 +26,15 @@ def _unpack(v: int):
     return int(v & 0xFFFFFFFF), int(v >> 32)
 
 
+class DeviceArray:
+    """Device memory of the library with a shape, for whatever reads ``__cuda_array_interface__`` (``torch.as_tensor``).  The
+    library's work on it is in order with the reader's on a stream lent with ``set_stream``; otherwise ``sync`` lies between."""
+
+    def __init__(self, owner, ptr: int, shape, typestr: str):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(shape), "typestr": typestr, "version": 2}
+
+
 class Adamah:
     def __init__(self, lib_path: Optional[str] = None, cache_mb: Optional[int] = None, cold_cache_mb: Optional[int] = None):
         self._lib = _lib.load()
@@ -33,6 +42,7 @@ class Adamah:
         if rc != 0:
             raise RuntimeError(f"adamah_init failed with code {rc}: {_lib.last_error()}")
         self._maps: Dict[int, tuple] = {}
+        self._kvs: Dict[int, KvDesc] = {}
         self._active_dtype = C.DTYPE_F32
         self._group_size = 32
         self._metrics = {"scatter_calls": 0, "gather_calls": 0, "total_bytes_cpu_to_gpu": 0, "total_bytes_gpu_to_cpu": 0}
@@ -308,6 +318,118 @@ class Adamah:
         self._check(self._lib.map_matvec_argmax_t_xq4_static_dev(map_act, map_wt, locs_a_handle, locs_b_handle, locs_idx_tmp_handle,
                                                                  locs_val_tmp_handle, locs_dst_handle, K, N, rows_per_group),
                     "map_matvec_argmax_t_xq4_static_dev")
+
+    # ---- paged key / value caches (extension) --------------------------------------------------
+    def kv_create(self, n_layer: int, n_head_kv: int, head_dim: int, n_pages: int, max_seqs: int, max_pages: int, page_size: int = 64,
+                  kv_dtype: str = "f16") -> int:
+        """A pool of pages of keys and values (``kv_dtype`` "f16" or "f32") and ``max_seqs`` empty sequences of up to
+        ``max_pages`` pages; returns the cache's id."""
+        if kv_dtype not in ("f32", "f16"):
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r}")
+        d = KvDesc(n_layer, n_head_kv, head_dim, ("f32", "f16").index(kv_dtype), page_size, n_pages, max_seqs, max_pages)
+        kid = ctypes.c_uint32(0)
+        self._check(self._lib.adam_b200_kv_create(ctypes.byref(d), ctypes.byref(kid)), "adam_b200_kv_create")
+        d.page_size = d.page_size or 64
+        self._kvs[int(kid.value)] = d
+        return int(kid.value)
+
+    def kv_destroy(self, kv: int):
+        self._check(self._lib.adam_b200_kv_destroy(kv), "adam_b200_kv_destroy")
+        self._kvs.pop(kv, None)
+
+    @staticmethod
+    def _counts(seqs, n):
+        """Sequences and a number for each as uint32 arrays; one number stands for all."""
+        seqs = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        n = np.ascontiguousarray(n, np.uint32).reshape(-1)
+        if n.size == 1 and seqs.size != 1:
+            n = np.full(seqs.size, n[0], np.uint32)
+        if n.size != seqs.size:
+            raise ValueError(f"{seqs.size} sequences, but {n.size} numbers")
+        return seqs, n
+
+    def kv_extend(self, kv: int, seqs, n_tokens):
+        """Room for ``n_tokens`` more positions of each sequence (a number, or one per sequence).  Shared pages that would be
+        written are replaced by copies first."""
+        seqs, n = self._counts(seqs, n_tokens)
+        self._check(self._lib.adam_b200_kv_extend(kv, seqs.size, seqs.ctypes.data, n.ctypes.data), "adam_b200_kv_extend")
+
+    def kv_fork(self, kv: int, src: int, dsts, n_tokens: Optional[int] = None):
+        """The empty sequences ``dsts`` share the first ``n_tokens`` positions of ``src`` (default: all of them)."""
+        dsts = np.ascontiguousarray(dsts, np.uint32).reshape(-1)
+        if n_tokens is None:
+            n_tokens = self.kv_lens(kv)[src]
+        self._check(self._lib.adam_b200_kv_fork(kv, src, dsts.size, dsts.ctypes.data, int(n_tokens)), "adam_b200_kv_fork")
+
+    def kv_truncate(self, kv: int, seqs, lens=0):
+        """Each sequence keeps its first ``lens`` positions (0: none); pages that nobody holds are free again."""
+        seqs, n = self._counts(seqs, lens)
+        self._check(self._lib.adam_b200_kv_truncate(kv, seqs.size, seqs.ctypes.data, n.ctypes.data), "adam_b200_kv_truncate")
+
+    def kv_compact(self, kv: int) -> int:
+        """Moves the held pages to the front of the pool; returns how many there are."""
+        live = ctypes.c_uint32(0)
+        self._check(self._lib.adam_b200_kv_compact(kv, ctypes.byref(live)), "adam_b200_kv_compact")
+        return int(live.value)
+
+    def _kv_desc(self, kv: int) -> KvDesc:
+        if kv not in self._kvs:
+            raise ValueError(f"kv cache {kv} does not exist")
+        return self._kvs[kv]
+
+    def kv_free_pages(self, kv: int) -> int:
+        n = ctypes.c_uint32(0)
+        self._check(self._lib.adam_b200_kv_state(kv, ctypes.byref(n), None, None), "adam_b200_kv_state")
+        return int(n.value)
+
+    def kv_lens(self, kv: int) -> np.ndarray:
+        """Positions of every sequence."""
+        out = np.empty(self._kv_desc(kv).max_seqs, np.int32)
+        self._check(self._lib.adam_b200_kv_state(kv, None, out.ctypes.data, None), "adam_b200_kv_state")
+        return out
+
+    def kv_table(self, kv: int) -> np.ndarray:
+        """Pages of every sequence, ``[max_seqs, max_pages]``, -1 where there is none."""
+        d = self._kv_desc(kv)
+        out = np.empty((d.max_seqs, d.max_pages), np.int32)
+        self._check(self._lib.adam_b200_kv_state(kv, None, None, out.ctypes.data), "adam_b200_kv_state")
+        return out
+
+    def kv_array(self, kv: int, which: str) -> DeviceArray:
+        """The cache's device memory: "pool" ``[n_pages, n_layer, 2, n_head_kv, page_size, head_dim]`` (keys, values), "table"
+        ``[max_seqs, max_pages]`` or "lens" ``[max_seqs]``."""
+        d = self._kv_desc(kv)
+        shape, kind = {"pool": ((d.n_pages, d.n_layer, 2, d.n_head_kv, d.page_size, d.head_dim), "<f2" if d.kv_dtype else "<f4"),
+                       "table": ((d.max_seqs, d.max_pages), "<i4"), "lens": ((d.max_seqs,), "<i4")}[which]
+        p, n = ctypes.c_uint64(), ctypes.c_uint64()
+        self._check(self._lib.adam_b200_kv_ptr(kv, ("pool", "table", "lens").index(which), ctypes.byref(p), ctypes.byref(n)), "adam_b200_kv_ptr")
+        return DeviceArray(self, int(p.value), shape, kind)
+
+    def map_array(self, map_id: int) -> DeviceArray:
+        """A float32 map's device memory."""
+        if self._maps.get(map_id, (0, 0, 0, None))[3] != C.DTYPE_F32:
+            raise ValueError(f"map {map_id} is not a float32 map")
+        p, n = ctypes.c_uint64(), ctypes.c_uint64()
+        self._check(self._lib.adam_b200_map_ptr(map_id, ctypes.byref(p), ctypes.byref(n)), "adam_b200_map_ptr")
+        return DeviceArray(self, int(p.value), (int(n.value) // 4,), "<f4")
+
+    def map_qk_norm_rope_kv_dev(self, map_act, map_wt, kv, layer, locs_q_handle, locs_k_handle, locs_v_handle, locs_q_wt_handle, locs_k_wt_handle,
+                                locs_q_dst_handle, seq_handle, start_handle, n_seqs, n_rows, n_head, freq_base=10000.0, eps=1e-6):
+        """Norm and rotation of the new rows' queries and keys, keys and values into the cache (0 for a weight handle: no norm)."""
+        self._check(self._lib.map_qk_norm_rope_kv_dev(map_act, map_wt, kv, layer, locs_q_handle, locs_k_handle, locs_v_handle, locs_q_wt_handle,
+                                                      locs_k_wt_handle, locs_q_dst_handle, seq_handle, start_handle, n_seqs, n_rows, n_head,
+                                                      freq_base, eps), "map_qk_norm_rope_kv_dev")
+
+    def map_attn_kv_dev(self, map_id, kv, layer, locs_q_handle, locs_out_handle, seq_handle, start_handle, n_seqs, n_rows, n_head, window=0,
+                        n_sink=0, scale=1.0, cap=0.0):
+        """Attention of the new rows over their sequences' pages, with a sliding window (0: none), first positions that stay
+        visible and a soft cap (0: none)."""
+        self._check(self._lib.map_attn_kv_dev(map_id, kv, layer, locs_q_handle, locs_out_handle, seq_handle, start_handle, n_seqs, n_rows, n_head,
+                                              window, n_sink, scale, cap), "map_attn_kv_dev")
+
+    def map_sample_dev(self, map_id, locs_logits_handle, rule_handle, locs_u_handle, locs_dst_handle, n_rows, n_vocab):
+        """A token per row of logits; ``rule_handle`` holds ``n_rows`` values of ``constants.SAMPLE_RULE``."""
+        self._check(self._lib.map_sample_dev(map_id, locs_logits_handle, rule_handle, locs_u_handle, locs_dst_handle, n_rows, n_vocab), "map_sample_dev")
 
     # ---- batching / fusion / stats -------------------------------------------------
     def batch_begin(self):

@@ -68,3 +68,8 @@ GGML_TYPE_Q8_0 = 8
 GGML_TYPE_Q4_K = 12
 # map dtype that stores each block type as it is in the file
 GGUF_MAP_DTYPE = {GGML_TYPE_Q4_0: DTYPE_GGUF_Q4_0, GGML_TYPE_Q4_K: DTYPE_GGUF_Q4_K, GGML_TYPE_Q8_0: DTYPE_GGUF_Q8_0, GGML_TYPE_Q5_0: DTYPE_GGUF_Q5_0}
+
+# fields of a sampling rule, a numpy dtype (adam_b200_sample_rule of include/adam_b200.h): what a rule_handle of map_sample_dev holds
+SAMPLE_RULE = [("temperature", "<f4"), ("top_k", "<u4"), ("top_p", "<f4"), ("min_p", "<f4")]
+# entry of a batch of sequences that stands for none (map_qk_norm_rope_kv_dev, map_attn_kv_dev)
+KV_NO_SEQ = 0xFFFFFFFF

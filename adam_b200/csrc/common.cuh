@@ -19,6 +19,7 @@ constexpr uint32_t MAX_HANDLES = 1u << 16; // reference: MAX_RES 2048 (adamah.c:
 constexpr uint32_t DEVERR_OOB_MAP   = 1u;   // a loc pointed outside its map
 constexpr uint32_t DEVERR_WAIT      = 2u;   // a bounded device-side wait ran out
 constexpr uint32_t DEVERR_BAD_TOKEN = 4u;   // token id outside the vocabulary
+constexpr uint32_t DEVERR_BAD_RULE  = 8u;   // a sampling rule or random number out of range
 
 struct Map {
     bool     used;

@@ -247,7 +247,7 @@ extern "C" int adamah_init_ex(uint64_t, uint64_t) {
 }
 extern "C" int adamah_init(void) { return adamah_init_ex(0, 0); }
 
-namespace ab { void decoder_destroy_all(); void plans_clear_all(); void tiled_drop_map(uint32_t map_id); void ar_destroy_all(); void gemm_tc_release(); void sample_free_all(); void file_stage_release(); }
+namespace ab { void decoder_destroy_all(); void plans_clear_all(); void tiled_drop_map(uint32_t map_id); void ar_destroy_all(); void gemm_tc_release(); void sample_free_all(); void file_stage_release(); void kv_destroy_all(); }
 
 static void io_release();
 extern "C" void adamah_shutdown(void) {
@@ -256,6 +256,7 @@ extern "C" void adamah_shutdown(void) {
     cudaStreamSynchronize(g.stream);
     ar_destroy_all();
     decoder_destroy_all();
+    kv_destroy_all();
     sample_free_all();
     file_stage_release();
     io_release();
@@ -309,7 +310,7 @@ extern "C" int adam_b200_step_kernel_counts(uint64_t* out, uint32_t n) {
     return ADAMAH_OK;
 }
 // Reads and clears the device error word (bits: 1 = a loc fell outside its map,
-// 2 = a bounded device wait ran out, 4 = bad token id).
+// 2 = a bounded device wait ran out, 4 = bad token id, 8 = bad sampling rule).
 extern "C" uint32_t adam_b200_device_error(void) {
     if (!g.inited) return 0;
     uint32_t v = 0;
@@ -407,6 +408,14 @@ extern "C" int map_init(uint32_t id, uint32_t word_size, uint32_t pack_size, uin
 
 extern "C" uint32_t map_size(uint32_t id) { Map* m = get_map(id); return m ? m->n_packs : 0; }
 extern "C" uint32_t map_get_dtype(uint32_t id) { Map* m = get_map(id); return m ? m->dtype : 0xFFFFFFFFu; }
+
+extern "C" int adam_b200_map_ptr(uint32_t id, uint64_t* ptr_out, uint64_t* bytes_out) {
+    Map* m = get_map(id);
+    if (!m) return ADAMAH_ERR_NOT_FOUND;
+    if (!ptr_out || !bytes_out) return fail(ADAMAH_ERR_INVALID, "map_ptr: null pointer");
+    *ptr_out = (uint64_t)(uintptr_t)m->buf; *bytes_out = m->bytes;
+    return ADAMAH_OK;
+}
 
 extern "C" int map_set_qparams(uint32_t id, const float* scales, const float* zeros, uint32_t n_groups) {
     Map* m = get_map(id);

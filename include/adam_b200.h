@@ -230,7 +230,8 @@ uint64_t    adam_b200_kernel_launches(void);
 int         adam_b200_step_kernel_counts(uint64_t* out, uint32_t n);
 
 /* Reads and clears the device error word: bit 0 = a loc fell outside its map,
- * bit 1 = a bounded device-side wait ran out, bit 2 = token id out of range.
+ * bit 1 = a bounded device-side wait ran out, bit 2 = token id out of range,
+ * bit 3 = a sampling rule or random number out of range.
  * Kernels record these instead of faulting. */
 uint32_t    adam_b200_device_error(void);
 /* Free a loc handle (the reference evicts instead: adamah.c:1328 res_evict_one). */
@@ -297,6 +298,84 @@ int map_matvec_argmax_t_xq4_static_dev(uint32_t map_act, uint32_t map_wt, uint32
  * integer; 0 = back to the library's own stream), so the caller's collectives or kernels on
  * that stream are ordered with the library's.  Synchronises the stream in use first. */
 int adam_b200_set_stream(uint64_t stream);
+
+/* Device address and size of a map's storage, for callers that fill a float32 map from, or hand its values to, kernels of
+ * their own.  The library's work on it is in order with the caller's on a stream lent with adam_b200_set_stream; otherwise
+ * adamah_sync lies between them.  Valid until the map is destroyed. */
+int adam_b200_map_ptr(uint32_t map, uint64_t* ptr_out, uint64_t* bytes_out);
+
+/* ---- paged key / value cache for callers that issue the operators themselves -------------------
+ * A pool of n_pages pages of page_size positions (keys and values of every layer), and max_seqs sequences that each hold up
+ * to max_pages of them.  A sequence is a number below max_seqs and has a length, 0 at first.  Which sequence holds which page
+ * is host arithmetic; what follows from it on the device is enqueued like an operator, with no wait.  Pages cannot change
+ * hands while a graph is being captured; a captured operator reads the lengths and pages of the time it is replayed, and must
+ * not be replayed once its cache is destroyed.  No counterpart in the reference (one contiguous cache per engine,
+ * adam/models/engine.py:3045-3302). */
+typedef struct adam_b200_kv_desc {
+    uint32_t n_layer, n_head_kv;
+    uint32_t head_dim;           /* 32, 64, 128 or 256 */
+    uint32_t kv_dtype;           /* 0 = float32, 1 = float16 */
+    uint32_t page_size;          /* positions per page, 1..1024 (0 -> 64) */
+    uint32_t n_pages, max_seqs, max_pages;
+} adam_b200_kv_desc;
+int adam_b200_kv_create(const adam_b200_kv_desc* desc, uint32_t* id_out);
+int adam_b200_kv_destroy(uint32_t id);
+/* Sequence seqs[i] grows by n_tokens[i] positions, whose keys and values are then the caller's to write
+ * (map_qk_norm_rope_kv_dev).  New pages are the lowest-numbered free ones, sequence after sequence.  A page that the sequence
+ * holds in part and shares is replaced by a copy of the positions it has there.  Every sequence once per call; all of them
+ * grow or, where pages run out (ADAMAH_ERR_MEMORY), none does. */
+int adam_b200_kv_extend(uint32_t id, uint32_t n, const uint32_t* seqs, const uint32_t* n_tokens);
+/* The empty sequences dsts[i] get the first n_tokens positions of src: its pages, shared, nothing is copied.  Positions
+ * below n_tokens cannot be written any more, by src neither. */
+int adam_b200_kv_fork(uint32_t id, uint32_t src, uint32_t n, const uint32_t* dsts, uint32_t n_tokens);
+/* Sequence seqs[i] keeps its first lens[i] positions (0: it is empty again); pages that no sequence holds are free. */
+int adam_b200_kv_truncate(uint32_t id, uint32_t n, const uint32_t* seqs, const uint32_t* lens);
+/* The held pages move to the front of the pool: the ones at or behind their number, ascending, to the free ones below it,
+ * ascending, each as a whole.  n_live_out: pages held. */
+int adam_b200_kv_compact(uint32_t id, uint32_t* n_live_out);
+/* Free pages, lengths [max_seqs] and page table [max_seqs][max_pages] (-1 = none) as the host has them; any may be NULL. */
+int adam_b200_kv_state(uint32_t id, uint32_t* n_free_out, int32_t* lens_out, int32_t* table_out);
+/* Device address / size of the pool [n_pages][n_layer][key, value][n_head_kv][page_size][head_dim] (which = 0), of the page
+ * table (1) and of the lengths (2); see adam_b200_map_ptr for the order of work. */
+int adam_b200_kv_ptr(uint32_t id, uint32_t which, uint64_t* ptr_out, uint64_t* bytes_out);
+
+/* Operators on the new rows of a batch of sequences.  Entry e of the batch is sequence seq_h[e] of the cache with the rows
+ * start_h[e] .. start_h[e + 1] - 1 (start_h has n_seqs + 1 values, ascending, the last at most n_rows); row r's queries, keys,
+ * values and results lie at the r-th offset of their handles, head by head.  An entry's rows are the last positions of its
+ * sequence: adam_b200_kv_extend comes first.  An entry 0xFFFFFFFF is no sequence; its rows, and rows outside every entry, are
+ * left as they are.  A sequence stands in one entry.  Trouble on the device (an offset outside its map, a position that the
+ * sequence does not have or may not write) sets bit 0 of the device error word and leaves the row out. */
+/* Every query and key head: RMS norm with the vector at qwt_h / kwt_h (one offset into map_wt; handle 0: no norm), rotation of
+ * the pairs (i, i + head_dim / 2) by position * freq_base^(-2 i / head_dim), angles in 64 bits (map_rope_dev's are rounded
+ * to 32).  Queries go to qdst_h (the rows at q_h or rows that nothing else of the call lies on), keys and values into the
+ * cache. */
+int map_qk_norm_rope_kv_dev(uint32_t map_act, uint32_t map_wt, uint32_t kv, uint32_t layer, uint32_t q_h, uint32_t k_h, uint32_t v_h,
+                            uint32_t qwt_h, uint32_t kwt_h, uint32_t qdst_h, uint32_t seq_h, uint32_t start_h, uint32_t n_seqs,
+                            uint32_t n_rows, uint32_t n_head, float freq_base, float eps);
+/* Attention of the rows' queries (q_h, n_head heads, already rotated) over their sequences' keys and values in the cache,
+ * results to out_h (rows that no queries of the call lie on, but for a row's own).  Position p attends to the positions j <= p,
+ * with a window only to the last `window` of them (its own among them) and to the first n_sink of the sequence.
+ * Scores are scale * q.k, or cap * tanh(scale * q.k / cap) where cap > 0. */
+int map_attn_kv_dev(uint32_t map, uint32_t kv, uint32_t layer, uint32_t q_h, uint32_t out_h, uint32_t seq_h, uint32_t start_h,
+                    uint32_t n_seqs, uint32_t n_rows, uint32_t n_head, uint32_t window, uint32_t n_sink, float scale, float cap);
+
+/* A token per row of logits (n_vocab values at the r-th offset of logits_h) by the row's own rule and random number.
+ * rule_h holds adam_b200_sample_rule[n_rows]; u_h one offset per row of a number in [0, 1); the token goes to dst_h's offset
+ * as float32, like every index (n_vocab at most 2^24).
+ * The weights are exp((logit - largest) / temperature).  In the order of falling logits, lower index first, the first top_k
+ * stay, of those the shortest run whose weights reach top_p of theirs, of those the ones with a weight of min_p or more; the
+ * first never goes.  The token is the lowest index whose running sum, in index order, is above u times the sum.  With
+ * temperature <= 0 the first is taken.  Weights are rounded to units of 2^-45 of the largest
+ * (2^-39 at 2^24 logits), sums of them are exact: what is drawn does not depend on the launch.  Logits of -infinity and NaN are never drawn; a row of
+ * nothing else gives -1.  Rules and numbers out of range (NaN, u outside [0, 1)) give -1 and set bit 3 of the device error
+ * word. */
+typedef struct adam_b200_sample_rule {
+    float    temperature;
+    uint32_t top_k;              /* 0: all */
+    float    top_p;              /* 1 and more: all */
+    float    min_p;              /* of the largest weight; 0: all */
+} adam_b200_sample_rule;
+int map_sample_dev(uint32_t map, uint32_t logits_h, uint32_t rule_h, uint32_t u_h, uint32_t dst_h, uint32_t n_rows, uint32_t n_vocab);
 
 /* ---- one-shot all-reduce over peer memory (tensor-parallel decode) -----------------
  * Sum of a small fp32 buffer over 2..8 ranks (one process per GPU of one node): every rank
