@@ -206,10 +206,15 @@ class _Held:
         self.maps.append(m)
         offs = np.cumsum([0] + [t.numel() for t in tensors]).tolist()
         self.gpu.map_create_typed(m, adam_b200.DTYPE_F32, 1, offs[-1] + extra)
-        view = torch.as_tensor(self.gpu.map_array(m), device="cuda")
+        view = self.view(self.gpu.map_array(m))
         for o, t in zip(offs, tensors):
             view[o:o + t.numel()] = t.reshape(-1)
         return m, offs, view
+
+    def view(self, array):
+        """A tensor over the library's memory; what it lies in lives as long as the tensor does."""
+        array.owner = self
+        return torch.as_tensor(array, device="cuda")
 
     def up(self, values):
         h, _ = self.gpu.upload_dev(np.ascontiguousarray(values))
@@ -247,10 +252,10 @@ def _hold(s):
             held.up((offs[2] + np.arange(R)).astype(np.uint32))
         return
     kv = s["kv"] = held.cache(s, case, case.get("layers", LAYERS))
-    pool = torch.as_tensor(g.kv_array(kv, "pool"), device="cuda")
+    pool = held.view(g.kv_array(kv, "pool"))
     pool.copy_(s["pool"])
     s["pool"] = pool
-    s["views"] = [torch.as_tensor(g.kv_array(kv, k), device="cuda") for k in ("table", "lens")]
+    s["views"] = [held.view(g.kv_array(kv, k)) for k in ("table", "lens")]
     if s["kind"] == "fork":
         g.kv_extend(kv, [0], [case["tokens"]])
         s["others"] = np.arange(1, case["seqs"] + 1, dtype=np.uint32)
