@@ -1,0 +1,194 @@
+// Attention over a paged cache: arguments and what the kernels of attn_kv.cu and attn_kv_tc.cu share.
+#pragma once
+#include "kv_cache.cuh"
+
+namespace ab {
+
+struct AttnArgs {
+    float* act; uint64_t n_act;
+    const uint32_t *l_q, *l_out;
+    KvBatch b; KvGeom geo; const void* pool;
+    uint32_t layer, n_head, group, window, n_sink;      // group: query heads of a key head
+    float scale, cap;
+    uint32_t splits, least;                             // CTAs that may share a tile's positions; chunks that one takes at least
+    float* part; unsigned int* tickets;
+    uint32_t* err;
+};
+
+// A row of a tile: an entry's rows times its group's heads, counted token by token, cut into tiles.
+struct AttnRow { uint64_t q, o; int32_t pos; };         // offsets of the head's values; pos < 0: no such row
+
+struct AttnTile {
+    uint32_t seq, row, n, first;                        // sequence, its first row of the batch and how many, first (row, head) of the tile
+    int32_t lo, hi;                                     // least and largest position of the tile's rows
+    const int32_t* pages;
+    uint32_t sinks, main0, chunks;                      // chunks of first positions, first chunk of the others, all together
+    int32_t from;                                       // positions below it are seen by none but as first ones
+};
+
+// Tile t of the batch, by the whole CTA (`scratch`: a word per warp and two more); false: there is none, or nothing to do.
+// Fills rows[0 .. ROWS).  CHUNK: positions per chunk.
+template <int ROWS, int CHUNK>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t t, uint32_t kvh, AttnTile& x, AttnRow* rows, uint32_t* scratch) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    uint32_t* const hit = scratch + warps;              // entry and tile of the entry; no tile: entry 0xFFFFFFFF
+    uint32_t before = 0;
+    if (tid == 0) hit[0] = KV_NO_SEQ;
+    for (uint32_t e0 = 0; e0 < a.b.n_seqs; e0 += blockDim.x) {
+        const uint32_t e = e0 + tid;
+        uint32_t n = 0;
+        if (e < a.b.n_seqs) {
+            const uint32_t s0 = a.b.start[e], s1 = a.b.start[e + 1];
+            n = s0 < s1 && s1 <= a.b.n_rows ? s1 - s0 : 0u;
+            if (s1 < s0 || s1 > a.b.n_rows) atomicOr(a.err, DEVERR_OOB_MAP);
+        }
+        const uint32_t tiles = (n * a.group + ROWS - 1) / ROWS;
+        uint32_t incl = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += v; }
+        __syncthreads();
+        if (lane == 31) scratch[warp] = incl;
+        __syncthreads();
+        uint32_t at = before + incl - tiles;
+        for (uint32_t w = 0; w < warps; ++w) { if (w < warp) at += scratch[w]; before += scratch[w]; }
+        if (at <= t && t < at + tiles) { hit[0] = e; hit[1] = t - at; }
+        if (before > t) break;
+    }
+    __syncthreads();
+    const uint32_t e = hit[0];
+    if (e == KV_NO_SEQ) return false;
+    x.seq = a.b.seq[e];
+    if (x.seq == KV_NO_SEQ) return false;
+    if (x.seq >= a.b.max_seqs) { if (tid == 0) atomicOr(a.err, DEVERR_OOB_MAP); return false; }
+    x.row = a.b.start[e]; x.n = a.b.start[e + 1] - x.row; x.first = hit[1] * ROWS;
+    x.pages = a.b.table + (size_t)x.seq * a.geo.max_pages;
+    const int32_t pos0 = a.b.lens[x.seq] - (int32_t)x.n;
+    const uint32_t last = min(x.first + ROWS, x.n * a.group) - 1;
+    x.lo = max(pos0 + (int32_t)(x.first / a.group), 0); x.hi = pos0 + (int32_t)(last / a.group);
+    for (uint32_t r = tid; r < ROWS; r += blockDim.x) {
+        AttnRow y{0, 0, -1};
+        const uint32_t f = x.first + r, tok = f / a.group, head = kvh * a.group + f % a.group;
+        if (f <= last) {
+            const uint64_t oq = a.l_q[x.row + tok], oo = a.l_out[x.row + tok], len = (uint64_t)a.n_head * a.geo.hd;
+            y.pos = pos0 + (int32_t)tok;
+            if (y.pos < 0 || oq + len > a.n_act || oo + len > a.n_act) { y.pos = -1; atomicOr(a.err, DEVERR_OOB_MAP); }
+            y.q = oq + (uint64_t)head * a.geo.hd; y.o = oo + (uint64_t)head * a.geo.hd;
+        }
+        rows[r] = y;
+    }
+    x.from = a.window && x.lo >= (int32_t)a.window ? x.lo - (int32_t)a.window + 1 : 0;
+    x.main0 = (uint32_t)x.from / CHUNK;
+    x.sinks = min((min(a.n_sink, (uint32_t)x.from) + CHUNK - 1) / CHUNK, x.main0);
+    x.chunks = x.hi < 0 ? 0u : x.sinks + (uint32_t)x.hi / CHUNK + 1 - x.main0;
+    __syncthreads();
+    return x.chunks > 0;
+}
+template <int CHUNK>
+__device__ __forceinline__ int32_t chunk_at(const AttnTile& x, uint32_t c) { return (int32_t)((c < x.sinks ? c : c - x.sinks + x.main0) * CHUNK); }
+
+__device__ __forceinline__ bool row_sees(const AttnArgs& a, int32_t pos, int32_t p) {
+    return p <= pos && (a.window == 0 || p > pos - (int32_t)a.window || (uint32_t)p < a.n_sink);
+}
+// Does every row of the tile see all of the n positions from p on?
+__device__ __forceinline__ bool tile_sees(const AttnArgs& a, const AttnTile& x, int32_t p, int32_t n) {
+    return p + n - 1 <= x.lo && (a.window == 0 || p > x.hi - (int32_t)a.window || (uint32_t)(p + n) <= a.n_sink);
+}
+// Where position p of the tile's sequence lies in the cache (its key; elements), or -1 where no row of the tile sees it.
+__device__ __forceinline__ int64_t tile_position(const AttnArgs& a, const AttnTile& x, uint32_t kvh, int32_t p) {
+    if (p > x.hi || (p < x.from && (uint32_t)p >= a.n_sink)) return -1;
+    const int32_t page = x.pages[(uint32_t)p / a.geo.page];
+    return page < 0 ? -1 : (int64_t)kv_index(a.geo, (uint32_t)page, a.layer, 0, kvh, (uint32_t)p % a.geo.page);
+}
+
+__device__ __forceinline__ uint32_t at_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes to shared memory, zeros where there is no source
+__device__ __forceinline__ void at_cp16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void at_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void at_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void at_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void at_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void at_mma_h(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void at_mma_t(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x as the sum of two 11-bit terms (22 bits of it, and exact where x has no more)
+__device__ __forceinline__ void at_split_t(float x, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+__device__ __forceinline__ void at_split_h(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h); lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// A power of two that brings the largest of a row's values (its magnitude `most`) into [2^7, 2^8), and its inverse: fp16 terms
+// then neither overflow nor lose bits of what counts.
+__device__ __forceinline__ void row_scale(float most, float& up, float& down) {
+    int ex = 0;
+    if (most > 0.f && most < 3.0e38f) ex = max(-120, min(120, 134 - (int)((__float_as_uint(most) >> 23) & 0xFFu)));
+    up = __uint_as_float((uint32_t)(127 + ex) << 23); down = __uint_as_float((uint32_t)(127 - ex) << 23);
+}
+// tanh(x): below 1/4 its power series (the first term left out is 9e-9 of the value), else 1 - 2 / (1 + e^2x).
+__device__ __forceinline__ float at_tanh_small(float x) {
+    const float y = x * x;
+    return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), x);
+}
+__device__ __forceinline__ float at_tanh(float x) {
+    const float d = 1.f + expf(fminf(2.f * x, 80.f));
+    return fabsf(x) < 0.25f ? at_tanh_small(x) : 1.f - div_by(2.f, d, rcp_newton(d));
+}
+
+// One row by a warp, positions one after the other, only those that it sees read: for rows in whose tile an infinity or a NaN
+// stands that they do not see (a weight of 0 times it is a NaN in the tiles' products).  Sums over 64 positions at a time.
+template <typename T, int HD>
+__device__ __noinline__ void attend_row(const AttnArgs& a, const AttnTile x, const AttnRow row, uint32_t kvh) {
+    constexpr int N = HD / 32;
+    const uint32_t lane = threadIdx.x & 31;
+    float q[N], o[N] = {}, m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] = a.act[row.q + lane * N + j];
+    for (int32_t t0 = 0; t0 <= row.pos; t0 += 64) {
+        float ob[N] = {}, lb = 0.f;
+        const float m0 = m;
+        for (int32_t t = t0; t < min(t0 + 64, row.pos + 1); ++t) {
+            if (!row_sees(a, row.pos, t)) continue;
+            const int64_t at = tile_position(a, x, kvh, t);
+            if (at < 0) continue;
+            const T* k_row = reinterpret_cast<const T*>(a.pool) + at + lane * N;
+            KvRow<T, N> k, v;
+            k.load(k_row);
+            v.load(k_row + (size_t)a.geo.n_kv * a.geo.page * HD);
+            float y[N], s = 0.f;
+            k.to_float(y);
+#pragma unroll
+            for (int j = 0; j < N; ++j) s = fmaf(q[j], y[j], s);
+            s = warp_sum(s) * a.scale;
+            if (a.cap > 0.f) s = a.cap * tanhf(s / a.cap);
+            const float mn = max_nan(m, s), alpha = m == mn ? 1.f : expf(m - mn), p = s == -INFINITY ? 0.f : expf(s - mn);
+            v.to_float(y);
+            lb = fmaf(lb, alpha, p);
+            m = mn;
+#pragma unroll
+            for (int j = 0; j < N; ++j) ob[j] = fmaf(p, y[j], ob[j] * alpha);
+        }
+        const float alpha = m0 == m ? 1.f : expf(m0 - m);
+        l = fmaf(l, alpha, lb);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = fmaf(o[j], alpha, ob[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) a.act[row.o + lane * N + j] = o[j] / l;
+}
+
+}  // namespace ab

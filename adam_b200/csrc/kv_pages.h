@@ -32,6 +32,11 @@ public:
         refs.assign(pages, 0); stamp.assign(seqs, 0);
     }
 
+    uint32_t longest() {                            // the largest length
+        if (stale) { most = 0; for (int32_t n : lens) most = std::max(most, (uint32_t)n); stale = false; }
+        return most;
+    }
+
     int extend(uint32_t n, const uint32_t* seqs, const uint32_t* n_tokens, KvUpdate& u) {
         if (int rc = check("kv_extend", seqs, n, n_tokens)) return rc;
         const uint64_t cap = (uint64_t)max_pages * page;
@@ -65,6 +70,7 @@ public:
             }
             for (uint32_t j = pages_for(len); j < pages_for(to); ++j) give(u, s, j, take());
             lens[s] = (int32_t)to;
+            most = std::max(most, to);
             add_len(u, s);
         }
         return PAGES_OK;
@@ -100,6 +106,7 @@ public:
             const uint32_t s = seqs[i], old = pages_for((uint32_t)lens[s]), now = pages_for(to[i]);
             if (to[i] == (uint32_t)lens[s]) continue;
             for (uint32_t j = now; j < old; ++j) { drop((uint32_t)at(s, j)); at(s, j) = -1; }
+            stale |= (uint32_t)lens[s] == most;
             lens[s] = (int32_t)to[i];
             own[s] = std::min(own[s], (int32_t)to[i]);
             if (now < old) u.recs.push_back(rec(REC_CLEAR, s, now, old, 0));
@@ -136,6 +143,8 @@ public:
 private:
     std::vector<uint32_t> refs, stamp;              // sequences that hold a page; of a sequence, the call that named it last
     uint32_t call = 0, first_free = 0;              // no page below first_free is free
+    uint32_t most = 0;                              // longest(), unless it is `stale`: then at least that
+    bool stale = false;
 
     uint32_t pages_for(uint64_t n) const { return (uint32_t)((n + page - 1) / page); }
     int32_t& at(uint32_t seq, uint32_t i) { return table[(size_t)seq * max_pages + i]; }

@@ -46,6 +46,7 @@ void kv_read(Cache* c, int32_t* table, int32_t* lens, int32_t* own, uint32_t* n_
     put(c->books.table, table); put(c->books.lens, lens); put(c->books.own, own); *n_free = c->books.n_free;
     put(c->pool, pool); put(c->table, d_table); put(c->lens, d_lens); put(c->own, d_own);
 }
+uint32_t kv_longest(Cache* c) { return c->books.longest(); }
 // position p of sequence s as the append operator writes it: refused below the first writable position
 int kv_write(Cache* c, uint32_t s, uint32_t p, int32_t value) {
     if (p >= (uint32_t)c->lens[s] || p < (uint32_t)c->own[s]) return -1;

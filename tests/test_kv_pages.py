@@ -69,7 +69,7 @@ def _holds(b, want):
         used |= set(table[s, :need].tolist())
         got = pool[table[s, :need]].reshape(-1)[:len(values)]
         assert got.tolist() == values, (s, got.tolist(), values)
-    assert n_free == b.n_pages - len(used)
+    assert n_free == b.n_pages - len(used) and b.lib.kv_longest(b.c) == max(len(v) for v in want)
     return table, lens, own, n_free, pool
 
 
