@@ -23,11 +23,11 @@ namespace ab {
 
 namespace cg = cooperative_groups;
 
-constexpr int SV_T = 1024, SV_W = SV_T / 32;
-constexpr uint32_t SV_BINS = 2048;
 constexpr uint32_t SV_SUBS = 256;                    // stretches of a CTA's share, a sum for each
 constexpr uint32_t SV_RESIDENT = 36864;              // logits that a CTA keeps in shared memory at most
-constexpr uint32_t SV_FEW = 2048;                    // candidates that one CTA sorts
+constexpr uint32_t SV_TABLE = 1024;
+constexpr int SV_T = 1024, SV_W = SV_T / 32;
+constexpr uint32_t SV_BINS = 2048, SV_FEW = 2048;    // bins; candidates that one CTA sorts
 
 struct SampleArgs {
     float* map; uint64_t n_el;
@@ -36,12 +36,13 @@ struct SampleArgs {
     uint32_t* err;
 };
 
-// A logit as an unsigned number in its order; both zeros are one.
-__device__ __forceinline__ uint32_t sv_key(float x) {
+// A logit and its index as a number that falls with the order of the rule; both zeros are one.
+__device__ __forceinline__ uint64_t sv_key(float x, uint32_t i) {
     const uint32_t u = __float_as_uint(x + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - i);
 }
-__device__ __forceinline__ float sv_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+__device__ __forceinline__ float sv_value(uint64_t key) { const uint32_t k = (uint32_t)(key >> 32); return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ uint32_t sv_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -54,29 +55,32 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v) {      // inclusiv
     return v;
 }
 
-// Weights as integers.  (max - x) / (T ln 2) = y is formed in two 32-bit words; 2^-y = 2^-k 2^(-i/256) (1 - s) with the table's
-// entry i, an integer k and s = 1 - 2^-r, |r| <= 1/512, whose series needs three terms.  s is known to 2^-24 of itself, so a
-// weight to 1e-10 of itself: what is drawn changes with probability 1e-7 or so, and the 64-bit exponential cost 60 us more
-// for 64 rows of 262144.
+// Weights as integers.  (max - x) / (T ln 2) = y is formed in two 32-bit words; 2^-y = 2^-k 2^(-i/1024) (1 - s) with the table's
+// entry i, an integer k and s = 1 - 2^-r, |r| <= 2^-11, whose series needs two terms (the third is 7e-12).  s is known to
+// 2^-24 of itself, so a weight to 1e-10 of itself: what is drawn changes with probability 1e-7 or so.  64 rows of 262144, no
+// cuts: 96 us with conversions and the order's keys in the loop, against %PLAIN% us; more with the 64-bit exponential.
 struct SvWeights {
-    const uint64_t* table;                            // 2^62 2^(-i/256)
+    const uint64_t* table;                            // 2^62 2^(-i/1024)
     float mx, c_hi, c_lo; int shift;
-    __device__ __forceinline__ uint64_t operator()(float x) const {
+    __device__ __noinline__ uint64_t special(float x) const {        // no finite difference, or nothing left of the weight
         if (x == mx) return 1ull << shift;
+        if (!(mx - x > 3.402823466e+38f) || mx > 3.402823466e+38f) return 0;
+        const double w = exp2(-(((double)mx - (double)x) * ((double)c_hi + (double)c_lo)));       // the difference of two logits overflows
+        return (uint64_t)__double2ull_rn(w * (double)(1ull << shift));
+    }
+    __device__ __forceinline__ uint64_t operator()(float x) const {
+        constexpr float MAGIC = 12582912.f;            // 1.5 x 2^23: the low bits of a sum with it are the nearest integer
         const float d = mx - x, b = d - mx, d_lo = (mx - (d - b)) + (-x - b);
-        float y = d * c_hi, y_lo = fmaf(d, c_hi, -y) + fmaf(d, c_lo, d_lo * c_hi);
-        if (d > 3.402823466e+38f) {                    // beyond 32 bits: a logit or the difference of two
-            const double e = ((double)mx - (double)x) * ((double)c_hi + (double)c_lo);
-            y = (float)e; y_lo = (float)(e - (double)y);
-        }
-        if (!(y < (float)(shift + 1))) return 0;       // below half a unit, or not a number (an infinite maximum)
-        const float t = rintf(y * 256.f), r = fmaf(t, -1.f / 256.f, y) + y_lo;
-        const int ti = (int)t;
-        const float z = r * 0.69314718055994530942f, s = z * (1.f - z * (0.5f - z * (1.f / 6.f)));
-        const uint64_t w = table[ti & 255];
-        const int64_t cut = (int64_t)(uint32_t)(w >> 32) * (int)(s * 4294967296.f);
-        const int sh = 62 - shift + (ti >> 8);
-        return ((w - (uint64_t)cut) + (1ull << (sh - 1))) >> sh;
+        const float y = d * c_hi;
+        if (!(y < (float)(shift + 1))) return special(x);            // below half a unit, or not a number
+        const float t = fmaf(y, (float)SV_TABLE, MAGIC);
+        const float r = fmaf(t - MAGIC, -1.f / SV_TABLE, y) + (fmaf(d, c_hi, -y) + fmaf(d, c_lo, d_lo * c_hi));
+        const float z = r * 0.69314718055994530942f, s = fmaf(z * z, -0.5f, z);
+        const uint32_t ti = __float_as_uint(t) & 0x3fffffu;
+        const uint64_t w = table[ti % SV_TABLE];
+        const int cut = __float_as_int(fmaf(s, 4294967296.f, MAGIC)) - __float_as_int(MAGIC);
+        const uint32_t sh = 62 - shift + ti / SV_TABLE;
+        return (w - (uint64_t)((int64_t)(int)(w >> 32) * cut) + (1ull << (sh - 1))) >> sh;
     }
 };
 
@@ -84,26 +88,58 @@ struct SvBins { uint32_t n[SV_BINS], lo[SV_BINS], hi[SV_BINS]; };      // counts
 struct SvShared {
     union { SvBins own; uint64_t list[SV_FEW]; };     // the CTA's histogram; the first CTA's candidates
     union { SvBins all; uint64_t w[SV_FEW]; };        // its share of the cluster's bins, merged; the candidates' weights
-    uint64_t table[256];
-    uint64_t seg_v, pass_v; uint32_t ties;            // weights of that share; of what is kept; logits equal to the threshold
-    uint32_t kmin, kmax, n_list, first; float max;
-    uint64_t sub_v[SV_SUBS], wv[SV_W + 1];
-    uint32_t sub_n[SV_SUBS]; float wmax[SV_W];
+    uint64_t table[SV_TABLE];
+    uint64_t seg_v, pass_v;                           // weight of that share; of what is kept
+    uint64_t kmin, kmax, least;                       // of the crossing bin; the last that is kept
+    uint32_t n_list, first; float max;
+    uint64_t sub_v[SV_SUBS], wv[SV_W];
+    float wmax[SV_W];
     uint64_t hit_above, hit_v; uint32_t hit_bin, hit_n, hit_count;
     uint64_t peer_v[16];
 };
 
-// n 64-bit keys (a power of two) into falling order, by the whole CTA
-__device__ __forceinline__ void sv_sort(uint64_t* key, uint32_t n) {
-    for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t half = size >> 1; half > 0; half >>= 1) {
+// The first m of the list into falling order by the whole CTA; zeros go last.  Up to 128 by counting the larger ones; beyond
+// that a bitonic network whose exchanges inside a warp need no wait (350 candidates, twice: 9 -> 2 us).
+__device__ __forceinline__ void sv_sort(uint64_t* key, uint32_t m) {
+    const uint32_t tid = threadIdx.x;
+    __syncthreads();
+    if (m <= 128) {
+        const uint64_t mine = tid < m ? key[tid] : 0;
+        uint32_t r = 0;
+        if (mine)
+#pragma unroll 8
+            for (uint32_t j = 0; j < m; ++j) r += key[j] > mine;
+        __syncthreads();
+        if (tid < m) key[tid] = 0;
+        __syncthreads();
+        if (mine) key[r] = mine;
+        __syncthreads();
+        return;
+    }
+    uint32_t n = 256;
+    while (n < m) n <<= 1;
+    for (uint32_t i = m + tid; i < n; i += SV_T) key[i] = 0;
+    for (uint32_t size = 32; size <= n; size <<= 1) {
+        for (uint32_t half = size >> 1; half >= 32; half >>= 1) {
             __syncthreads();
-            for (uint32_t t = threadIdx.x; t < n / 2; t += SV_T) {
+            for (uint32_t t = tid; t < n / 2; t += SV_T) {
                 const uint32_t i = 2 * t - (t & (half - 1)), j = i + half;
                 const uint64_t x = key[i], y = key[j];
                 if ((x < y) == ((i & size) == 0)) { key[i] = y; key[j] = x; }
             }
         }
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += SV_T) {       // whole warps: n and SV_T are multiples of 32
+            uint64_t x = key[i];
+            for (uint32_t sz = size == 32 ? 2 : size; sz <= size; sz <<= 1)
+                for (uint32_t half = min(sz >> 1, 16u); half > 0; half >>= 1) {
+                    const uint64_t y = __shfl_xor_sync(0xffffffffu, x, half);
+                    const bool larger = ((i & half) == 0) == ((i & sz) == 0);      // this one of the two keeps the larger
+                    x = larger == (x > y) ? x : y;
+                }
+            key[i] = x;
+        }
+    }
     __syncthreads();
 }
 
@@ -115,38 +151,32 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     cg::cluster_group cl = cg::this_cluster();
     const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / C;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto together = [&]() { if (C == 1) __syncthreads(); else cl.sync(); };
     const uint64_t ol = a.l_logits[row], ou = a.l_u[row], od = a.l_dst[row];
+    const adam_b200_sample_rule rule = a.rules[row];
     const bool lead = rank == 0 && tid == 0;
     if (ol + a.V > a.n_el || ou >= a.n_el || od >= a.n_el) { if (lead) atomicOr(a.err, DEVERR_OOB_MAP); return; }
-    const adam_b200_sample_rule rule = a.rules[row];
     const float u = a.map[ou];
-    if (!(u >= 0.f && u < 1.f) || rule.temperature != rule.temperature || rule.top_p != rule.top_p || rule.min_p != rule.min_p) {
-        if (lead) { a.map[od] = -1.f; atomicOr(a.err, DEVERR_BAD_RULE); }
-        return;
-    }
     const uint32_t base = rank * a.chunk, n = base < a.V ? min(a.chunk, a.V - base) : 0u;
     const float* src = a.map + ol + base;
     const bool aligned = ((ol + base) & 3) == 0;
-    auto clean = [](float x) { return x == x ? x : -INFINITY; };
-    auto get = [&](uint32_t i) { return RES ? sx[i] : clean(src[i]); };
-    // f(logit, its place in the CTA's share) for each, in no order
+    const float* const at = RES ? sx : src;
+    // f(logit, its place in the CTA's share) for each, in no order.  A NaN fails every comparison below, like what is not kept.
     auto each = [&](auto f) {
         if (RES || aligned) {
-            const float4* v4 = reinterpret_cast<const float4*>(RES ? sx : src);
+            const float4* v4 = reinterpret_cast<const float4*>(at);
             const uint32_t n4 = n / 4;
 #pragma unroll 4
             for (uint32_t i = tid; i < n4; i += SV_T) {
                 const float4 v = v4[i];
-                f(clean(v.x), 4 * i); f(clean(v.y), 4 * i + 1); f(clean(v.z), 4 * i + 2); f(clean(v.w), 4 * i + 3);
+                f(v.x, 4 * i); f(v.y, 4 * i + 1); f(v.z, 4 * i + 2); f(v.w, 4 * i + 3);
             }
-            if (tid < n % 4) f(get(4 * n4 + tid), 4 * n4 + tid);
+            if (tid < n % 4) f(at[4 * n4 + tid], 4 * n4 + tid);
         } else {
 #pragma unroll 8
-            for (uint32_t i = tid; i < n; i += SV_T) f(clean(src[i]), i);
+            for (uint32_t i = tid; i < n; i += SV_T) f(at[i], i);
         }
     };
-    if (tid < 256) s.table[tid] = (uint64_t)__double2ull_rn(exp2(-(double)tid / 256.0) * 4611686018427387904.0);
-    if (tid == 0) { s.n_list = 0; s.first = 0xffffffffu; }
 
     // ---- the largest logit ----
     float mx = -INFINITY;
@@ -154,39 +184,44 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint32_t n4 = n / 4;
 #pragma unroll 4
         for (uint32_t i = tid; i < n4; i += SV_T) {
-            float4 v = reinterpret_cast<const float4*>(src)[i];
-            v.x = clean(v.x); v.y = clean(v.y); v.z = clean(v.z); v.w = clean(v.w);
+            const float4 v = reinterpret_cast<const float4*>(src)[i];
             reinterpret_cast<float4*>(sx)[i] = v;
             mx = fmaxf(fmaxf(mx, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
         }
-        if (tid < n % 4) { const float v = clean(src[4 * n4 + tid]); sx[4 * n4 + tid] = v; mx = fmaxf(mx, v); }
+        if (tid < n % 4) { const float v = src[4 * n4 + tid]; sx[4 * n4 + tid] = v; mx = fmaxf(mx, v); }
     } else if (RES) {
 #pragma unroll 8
-        for (uint32_t i = tid; i < n; i += SV_T) { const float v = clean(src[i]); sx[i] = v; mx = fmaxf(mx, v); }
+        for (uint32_t i = tid; i < n; i += SV_T) { const float v = src[i]; sx[i] = v; mx = fmaxf(mx, v); }
     } else
         each([&](float x, uint32_t) { mx = fmaxf(mx, x); });
+    if (!(u >= 0.f && u < 1.f) || rule.temperature != rule.temperature || rule.top_p != rule.top_p || rule.min_p != rule.min_p) {
+        if (lead) { a.map[od] = -1.f; atomicOr(a.err, DEVERR_BAD_RULE); }
+        return;
+    }
     mx = warp_max(mx);
     if (lane == 0) s.wmax[warp] = mx;
+    if (tid == 0) { s.n_list = 0; s.first = 0xffffffffu; }
     __syncthreads();
     if (warp == 0) {
         mx = warp_max(s.wmax[lane]);
         if (lane == 0) s.max = mx;
     }
-    cl.sync();
+    together();
     mx = -INFINITY;
     for (uint32_t c = 0; c < C; ++c) mx = fmaxf(mx, *cl.map_shared_rank(&s.max, c));
     if (mx == -INFINITY || !(rule.temperature > 0.f)) {         // nothing to draw, or the first of the largest: the cluster agrees
         if (mx == -INFINITY) { if (lead) a.map[od] = -1.f; }
         else {
-            uint32_t at = 0xffffffffu;
-            each([&](float x, uint32_t i) { if (x == mx) at = min(at, i); });
-            at = __reduce_min_sync(0xffffffffu, at);
-            if (lane == 0 && at != 0xffffffffu) atomicMin(cl.map_shared_rank(&s.first, 0), base + at);
+            uint32_t i0 = 0xffffffffu;
+            each([&](float x, uint32_t i) { if (x == mx) i0 = min(i0, i); });
+            i0 = __reduce_min_sync(0xffffffffu, i0);
+            if (lane == 0 && i0 != 0xffffffffu) atomicMin(cl.map_shared_rank(&s.first, 0), base + i0);
         }
-        cl.sync();
+        together();
         if (lead && mx != -INFINITY) a.map[od] = (float)s.first;
         return;
     }
+    for (uint32_t i = tid; i < SV_TABLE; i += SV_T) s.table[i] = (uint64_t)__double2ull_rn(exp2(-(double)i / SV_TABLE) * 4611686018427387904.0);
 
     const double c = 1.4426950408889634074 / (double)rule.temperature;
     const float c_hi = (float)c;
@@ -194,19 +229,20 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     const float step = 64.0f / rule.temperature;
     const uint64_t least = (uint64_t)ceil((double)fminf(fmaxf(rule.min_p, 0.f), 1.f) * (double)(1ull << a.shift));    // of min_p
     auto bin_of = [&](float x) -> uint32_t {
-        if (x == mx) return 0u;
         const float t = (mx - x) * step;
-        return t < (float)(SV_BINS - 1) ? (uint32_t)t : SV_BINS - 1;
+        return t < (float)(SV_BINS - 1) ? (uint32_t)t : x == mx ? 0u : SV_BINS - 1;
     };
 
-    // ---- thresholds: a logit is kept if its key is above key_t, or equals it and it is one of the first n_ties of those ----
-    const uint32_t key_none = sv_key(-INFINITY);
-    uint32_t key_t = key_none, n_ties = 0;
+    // ---- the threshold: what is kept are the logits above x_t, and those equal to it up to index i_t ----
+    float x_t = -INFINITY;
+    uint32_t i_t = 0;
+    bool whole = true;                                // no cut yet: all but -infinity (and NaN)
+    auto kept = [&](float x, uint32_t i) { return x > x_t || (x == x_t && !whole && base + i <= i_t); };
 
     // The cluster's histogram: CTA c ends with the bins c * per .. of all, and their totals.
     const uint32_t per = SV_BINS / C;
     auto merge = [&](bool sums) {
-        cl.sync();
+        together();
         uint64_t tv = 0;
         for (uint32_t b = tid; b < per; b += SV_T) {
             uint32_t cn = 0; uint64_t cv = 0;
@@ -227,25 +263,31 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
             tv = warp_sum_u64(s.wv[lane]);
             if (lane == 0) s.seg_v = tv;
         }
-        cl.sync();
+        together();
         if (tid < C) s.peer_v[tid] = *cl.map_shared_rank(&s.seg_v, tid);
         __syncthreads();
     };
     auto total = [&]() { uint64_t v = 0; for (uint32_t k = 0; k < C; ++k) v += s.peer_v[k]; return v; };
+    // exclusive sums over the CTA, and the sum of all
+    auto scan = [&](uint64_t v, uint64_t& sum) {
+        const uint64_t incl = warp_scan_u64(v);
+        __syncthreads();
+        if (lane == 31) s.wv[warp] = incl;
+        __syncthreads();
+        const uint64_t ahead = warp_scan_u64(s.wv[lane]);
+        sum = __shfl_sync(0xffffffffu, ahead, 31);
+        const uint64_t before = __shfl_sync(0xffffffffu, ahead, warp ? warp - 1 : 0);
+        return incl - v + (warp ? before : 0ull);
+    };
     // The bin in which the running sum reaches `target` (1 .. total), the sum ahead of it, its own and its count: in s.hit_*.
     auto cross = [&](uint64_t target) {
-        uint64_t above = 0; uint32_t seg = 0;
+        uint64_t above = 0, sum; uint32_t seg = 0;
         while (seg + 1 < C && above + s.peer_v[seg] < target) above += s.peer_v[seg++];
         const SvBins* h = cl.map_shared_rank(&s.all, seg);
         const uint32_t mine = (per + SV_T - 1) / SV_T, b0 = tid * mine;
         uint64_t v = 0;
         for (uint32_t b = b0; b < min(b0 + mine, per); ++b) v += (uint64_t)h->lo[b] + ((uint64_t)h->hi[b] << 32);
-        const uint64_t incl = warp_scan_u64(v);
-        if (lane == 31) s.wv[warp] = incl;
-        __syncthreads();
-        const uint64_t ahead = warp_scan_u64(s.wv[lane]);
-        if (warp) above += __shfl_sync(0xffffffffu, ahead, warp - 1);
-        above += incl - v;
+        above += scan(v, sum);
         if (above < target && target <= above + v)
             for (uint32_t b = b0; b < min(b0 + mine, per); ++b) {
                 const uint64_t x = (uint64_t)h->lo[b] + ((uint64_t)h->hi[b] << 32);
@@ -254,8 +296,8 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
             }
         __syncthreads();
     };
-    auto clear = [&]() {
-        for (uint32_t b = tid; b < SV_BINS; b += SV_T) { s.own.n[b] = 0; s.own.lo[b] = 0; s.own.hi[b] = 0; }
+    auto clear = [&](bool sums) {
+        for (uint32_t b = tid; b < SV_BINS; b += SV_T) { s.own.n[b] = 0; if (sums) { s.own.lo[b] = 0; s.own.hi[b] = 0; } }
         __syncthreads();
     };
     auto count = [&](uint32_t b, float x, bool sums) {
@@ -270,184 +312,167 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint64_t p = (uint64_t)((double)fmaxf(rule.top_p, 0.f) * 18446744073709551616.0), t = __umul64hi(p, all) + (p * all != 0 ? 1u : 0u);
         return t ? t : 1ull;
     };
-    // Up to SV_FEW candidates in the first CTA's list: sorted, cut by the whole rule and drawn from there.  top_p is a share of
-    // `all`, or of the first top_k (all = 0).
+    // The logits for which `take` says so into the first CTA's list, sorted (SV_FEW at most).
+    auto collect = [&](auto take) {
+        uint32_t* const n_list = cl.map_shared_rank(&s.n_list, 0);
+        uint64_t* const list = cl.map_shared_rank(&s.list[0], 0);
+        each([&](float x, uint32_t i) { if (take(x, i)) list[atomicAdd(n_list, 1u)] = sv_key(x, base + i); });
+        together();
+        if (rank == 0) sv_sort(s.list, s.n_list);
+    };
+    constexpr int PER = SV_FEW / SV_T;                      // candidates of a thread
+    // All candidates in the list: cut by the whole rule and drawn from there.  top_p is a share of `all`, or of the first
+    // top_k (all = 0).
     auto few = [&](uint64_t all) {
-        const uint32_t m = s.n_list;
-        uint32_t size = 2;
-        while (size < m) size <<= 1;
-        for (uint32_t i = m + tid; i < size; i += SV_T) s.list[i] = 0;
-        sv_sort(s.list, size);                        // by key, then the lower index first
-        const uint32_t cand = rule.top_k > 0 ? min(m, rule.top_k) : m;
-        constexpr int PER = SV_FEW / SV_T;
-        uint64_t w[PER], mine = 0;
+        const uint32_t m = s.n_list, cand = rule.top_k > 0 ? min(m, rule.top_k) : m;
+        uint64_t w[PER], mine = 0, sum;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const uint32_t i = tid * PER + j;
-            w[j] = i < cand ? weight(sv_value((uint32_t)(s.list[i] >> 32))) : 0;
+            w[j] = i < cand ? weight(sv_value(s.list[i])) : 0;
             mine += w[j];
         }
-        auto scan = [&](uint64_t v, uint64_t& sum) {   // exclusive over the CTA
-            const uint64_t incl = warp_scan_u64(v);
-            __syncthreads();
-            if (lane == 31) s.wv[warp] = incl;
-            __syncthreads();
-            const uint64_t ahead = warp_scan_u64(s.wv[lane]);
-            sum = __shfl_sync(0xffffffffu, ahead, 31);
-            const uint64_t before = __shfl_sync(0xffffffffu, ahead, warp ? warp - 1 : 0);
-            return incl - v + (warp ? before : 0ull);
-        };
-        uint64_t sum, at = scan(mine, sum);
+        uint64_t ahead = scan(mine, sum);
         const uint64_t stop = rule.top_p < 1.f ? share(all ? all : sum) : ~0ull;      // kept while the sum ahead is below it
         // the kept ones again, by index
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const uint32_t i = tid * PER + j;
-            const bool in = i < cand && (i == 0 || at < stop) && w[j] >= least;
-            at += w[j];
-            const uint64_t e = i < m ? s.list[i] : 0;
-            if (i < SV_FEW) s.w[i] = w[j];
-            if (i < size) s.list[i] = in ? (e << 32) | i : 0;         // the low word of an entry falls with the index
+            const bool in = i < cand && (i == 0 || ahead < stop) && w[j] >= least;
+            ahead += w[j];
+            s.w[i] = w[j];
+            if (i < m) s.list[i] = in ? s.list[i] << 32 | i : 0;
         }
-        sv_sort(s.list, size);
+        sv_sort(s.list, m);
         mine = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const uint32_t i = tid * PER + j;
-            const uint64_t e = i < size ? s.list[i] : 0;
-            w[j] = e ? s.w[(uint32_t)e & (SV_FEW - 1)] : 0;
+            const uint64_t e = i < m ? s.list[i] : 0;
+            w[j] = e ? s.w[(uint32_t)e] : 0;
             mine += w[j];
         }
-        at = scan(mine, sum);
+        ahead = scan(mine, sum);
         const uint64_t target = __umul64hi((uint64_t)((double)u * 18446744073709551616.0), sum);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            if (at <= target && target < at + w[j]) a.map[od] = (float)(0xffffffffu - (uint32_t)(s.list[tid * PER + j] >> 32));
-            at += w[j];
+            if (ahead <= target && target < ahead + w[j]) a.map[od] = (float)(0xffffffffu - (uint32_t)(s.list[tid * PER + j] >> 32));
+            ahead += w[j];
         }
     };
     // Cuts what is kept to the run that reaches a target: so many logits (sums false), or so much weight.  True: the token is drawn.
     auto cut = [&](bool sums) -> bool {
-        clear();
-        each([&](float x, uint32_t) { if (sv_key(x) > key_t) count(bin_of(x), x, sums); });
+        clear(sums);
+        each([&](float x, uint32_t i) { if (kept(x, i)) count(bin_of(x), x, sums); });
         merge(sums);
-        const uint64_t above = total();               // of what lies above key_t; the ties at it are n_ties times one weight
-        uint64_t target;
-        if (sums) {
-            const uint64_t wt = n_ties ? weight(sv_value(key_t)) : 0;
-            target = share(above + n_ties * wt);
-            if (target > above) { n_ties = (uint32_t)((target - above + wt - 1) / wt); return false; }
-        } else {
-            if (above <= rule.top_k) return false;
-            target = rule.top_k;
-        }
+        const uint64_t all = total();
+        if (!sums && all <= rule.top_k) return false;
+        const uint64_t target = sums ? share(all) : rule.top_k;
         cross(target);
-        uint32_t in = s.hit_n;
         const uint32_t bin = s.hit_bin;
         uint64_t rest = target - s.hit_above;
-        // how many candidates lie in the bins up to it: where the first CTA can sort them, it does the rest
-        const uint32_t key_before = key_t, ties_before = n_ties;
-        if (ties_before == 0 && key_before == key_none) {
+        uint32_t in = s.hit_n;
+        if (whole) {
+            // how many candidates lie in the bins up to it: where the first CTA can sort them, it does the rest
             uint64_t upto = s.hit_above + s.hit_v;
-            if (sums) {                               // counts of the bins before it, this CTA's share of them
+            if (sums) {
                 uint32_t v = 0;
                 for (uint32_t b = tid; b < per; b += SV_T) v += rank * per + b <= bin ? s.all.n[b] : 0u;
                 v = __reduce_add_sync(0xffffffffu, v);
                 if (tid == 0) s.hit_count = 0;
                 __syncthreads();
                 if (lane == 0) atomicAdd(&s.hit_count, v);
-                cl.sync();
+                together();
                 upto = 0;
                 for (uint32_t k = 0; k < C; ++k) upto += *cl.map_shared_rank(&s.hit_count, k);
             }
             if (upto <= SV_FEW) {
-                uint32_t* const n_list = cl.map_shared_rank(&s.n_list, 0);
-                uint64_t* const list = cl.map_shared_rank(&s.list[0], 0);
-                each([&](float x, uint32_t i) {
-                    if (x > -INFINITY && bin_of(x) <= bin) list[atomicAdd(n_list, 1u)] = (uint64_t)sv_key(x) << 32 | (0xffffffffu - (base + i));
-                });
-                cl.sync();
-                if (rank == 0) few(sums ? above : 0);
+                collect([&](float x, uint32_t) { return x > -INFINITY && bin_of(x) <= bin; });
+                if (rank == 0) few(sums ? all : 0);
                 return true;
             }
         }
-        // the keys of the bin
-        uint32_t lo = 0xffffffffu, hi = 0u;
-        each([&](float x, uint32_t) {
-            const uint32_t k = sv_key(x);
-            if (k > key_t && bin_of(x) == bin) { lo = min(lo, k); hi = max(hi, k); }
-        });
-        lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
-        if (tid == 0) { s.kmin = 0xffffffffu; s.kmax = 0u; }
-        __syncthreads();
-        if (lane == 0) { atomicMin(&s.kmin, lo); atomicMax(&s.kmax, hi); }
-        cl.sync();
-        lo = 0xffffffffu; hi = 0u;
-        for (uint32_t k = 0; k < C; ++k) { lo = min(lo, *cl.map_shared_rank(&s.kmin, k)); hi = max(hi, *cl.map_shared_rank(&s.kmax, k)); }
-        for (;;) {
-            if (sums ? in == 1 : rest == in) { key_t = lo - 1; n_ties = 0; return false; }       // all of them
-            if (lo == hi) {
-                if (sums) { const uint64_t w = weight(sv_value(lo)); rest = (rest + w - 1) / w; }
-                key_t = lo; n_ties = (uint32_t)rest;
-                if (n_ties == in) { key_t = lo - 1; n_ties = 0; }
-                return false;
+        // The crossing bin, then the crossing one of 2048 equal pieces of the range of its logits' keys, and so on until the first
+        // CTA can sort what is left (logits that are all equal are told apart by their indices).
+        uint64_t lo = 0, hi = ~0ull;
+        bool ranged = false;
+        auto inside = [&](float x, uint32_t i) {
+            if (!kept(x, i) || bin_of(x) != bin) return false;
+            if (!ranged) return true;
+            const uint64_t k = sv_key(x, base + i);
+            return k >= lo && k <= hi;
+        };
+        while (in > SV_FEW) {
+            if (!ranged) {
+                uint64_t k0 = ~0ull, k1 = 0;
+                each([&](float x, uint32_t i) { if (inside(x, i)) { const uint64_t k = sv_key(x, base + i); k0 = min(k0, k); k1 = max(k1, k); } });
+                if (tid == 0) { s.kmin = ~0ull; s.kmax = 0; }
+                __syncthreads();
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) { k0 = min(k0, __shfl_xor_sync(0xffffffffu, k0, o)); k1 = max(k1, __shfl_xor_sync(0xffffffffu, k1, o)); }
+                if (lane == 0) { atomicMin((unsigned long long*)&s.kmin, (unsigned long long)k0); atomicMax((unsigned long long*)&s.kmax, (unsigned long long)k1); }
+                together();
+                lo = ~0ull; hi = 0;
+                for (uint32_t k = 0; k < C; ++k) { lo = min(lo, *cl.map_shared_rank(&s.kmin, k)); hi = max(hi, *cl.map_shared_rank(&s.kmax, k)); }
+                ranged = true;
             }
-            const int sh = max(0, 32 - __clz(hi - lo) - 11);
-            clear();
-            each([&](float x, uint32_t) {
-                const uint32_t k = sv_key(x);
-                if (k >= lo && k <= hi) count((hi - k) >> sh, x, sums);
-            });
+            const int sh = max(0, 64 - __clzll(hi - lo) - (11));
+            clear(sums);
+            each([&](float x, uint32_t i) { if (inside(x, i)) count((uint32_t)((hi - sv_key(x, base + i)) >> sh), x, sums); });
             merge(sums);
             cross(rest);
             in = s.hit_n; rest -= s.hit_above;
-            hi -= s.hit_bin << sh;
-            const uint32_t span = (1u << sh) - 1u;
+            hi -= (uint64_t)s.hit_bin << sh;
+            const uint64_t span = (1ull << sh) - 1u;
             lo = hi - lo > span ? hi - span : lo;
         }
+        collect(inside);
+        if (rank == 0) {
+            uint64_t w[PER], mine = 0, sum;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const uint32_t i = tid * PER + j;
+                w[j] = i < s.n_list ? (sums ? weight(sv_value(s.list[i])) : 1ull) : 0;
+                mine += w[j];
+            }
+            uint64_t ahead = scan(mine, sum);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (ahead < rest && rest <= ahead + w[j]) s.least = s.list[tid * PER + j];
+                ahead += w[j];
+            }
+            if (tid == 0) s.n_list = 0;
+        }
+        together();
+        const uint64_t k = *cl.map_shared_rank(&s.least, 0);
+        x_t = sv_value(k); i_t = sv_index(k); whole = false;
+        return false;
     };
     if (rule.top_k > 0 && rule.top_k < a.V && cut(false)) return;
     if (rule.top_p < 1.f && cut(true)) return;
+    __syncthreads();                                  // the table, where nothing was cut
 
     // ---- the draw: sums of stretches in index order, then the stretch that holds the token ----
-    const uint32_t sub = max(32u, ((a.chunk + SV_SUBS - 1) / SV_SUBS + 31) & ~31u), n_sub = (n + sub - 1) / sub;
-    const bool ranked = n_ties > 0;
-    uint32_t ties_before = 0;
-    if (ranked) {
-        for (uint32_t b = warp; b < n_sub; b += SV_W) {
-            uint32_t k = 0;
-            for (uint32_t i = b * sub + lane; i < (b + 1) * sub; i += 32) k += i < n && sv_key(get(i)) == key_t;
-            k = __reduce_add_sync(0xffffffffu, k);
-            if (lane == 0) s.sub_n[b] = k;
-        }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t t = 0;
-            for (uint32_t b = 0; b < n_sub; ++b) { const uint32_t k = s.sub_n[b]; s.sub_n[b] = t; t += k; }
-            s.ties = t;
-        }
-        cl.sync();
-        for (uint32_t k = 0; k < rank; ++k) ties_before += *cl.map_shared_rank(&s.ties, k);
-    }
-    // the weight of element i where it is kept; `tie`: its place among the equal ones (called by whole warps)
-    auto kept = [&](uint32_t i, uint32_t& tie) -> uint64_t {
-        const float x = i < n ? get(i) : -INFINITY;
-        const uint32_t k = sv_key(x);
-        bool in = k > key_t;
-        if (ranked) {
-            const uint32_t eq = __ballot_sync(0xffffffffu, k == key_t);
-            in |= k == key_t && tie + __popc(eq & ((1u << lane) - 1u)) < n_ties;
-            tie += __popc(eq);
-        }
-        if (!in) return 0;
+    const uint32_t sub = max(128u, ((a.chunk + SV_SUBS - 1) / SV_SUBS + 127) & ~127u), n_sub = (n + sub - 1) / sub;
+    auto value = [&](float x, uint32_t i) -> uint64_t {
+        if (!kept(x, i)) return 0;
         const uint64_t w = weight(x);
         return w >= least ? w : 0;
     };
     for (uint32_t b = warp; b < n_sub; b += SV_W) {
         uint64_t v = 0;
-        uint32_t tie = ranked ? ties_before + s.sub_n[b] : 0;
+        const uint32_t end = min(n, (b + 1) * sub);
+        if (RES || aligned) {
+#pragma unroll 2
+            for (uint32_t i = b * sub + 4 * lane; i + 3 < end; i += 128) {
+                const float4 x = *reinterpret_cast<const float4*>(at + i);
+                v += value(x.x, i) + value(x.y, i + 1) + value(x.z, i + 2) + value(x.w, i + 3);
+            }
+            if (const uint32_t i = (end & ~3u) + lane; i < end) v += value(at[i], i);
+        } else {
 #pragma unroll 4
-        for (uint32_t i = b * sub; i < (b + 1) * sub; i += 32) v += kept(i + lane, tie);
+            for (uint32_t i = b * sub + lane; i < end; i += 32) v += value(at[i], i);
+        }
         v = warp_sum_u64(v);
         if (lane == 0) s.sub_v[b] = v;
     }
@@ -458,7 +483,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         v = warp_sum_u64(v);
         if (lane == 0) s.pass_v = v;
     }
-    cl.sync();
+    together();
     uint64_t before = 0, all = 0;
     for (uint32_t k = 0; k < C; ++k) { const uint64_t v = *cl.map_shared_rank(&s.pass_v, k); before += k < rank ? v : 0; all += v; }
     const uint64_t target = __umul64hi((uint64_t)((double)u * 18446744073709551616.0), all);     // the running sum to be exceeded
@@ -466,25 +491,40 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         uint64_t v[SV_SUBS / 32], mine = 0;                        // lane l: stretches 8 l ..
 #pragma unroll
         for (int j = 0; j < (int)SV_SUBS / 32; ++j) { const uint32_t b = lane * (SV_SUBS / 32) + j; v[j] = b < n_sub ? s.sub_v[b] : 0; mine += v[j]; }
-        uint64_t at = before + warp_scan_u64(mine) - mine;
+        uint64_t ahead = before + warp_scan_u64(mine) - mine;
         uint32_t hit = 0xffffffffu;
 #pragma unroll
-        for (int j = 0; j < (int)SV_SUBS / 32; ++j) { if (hit == 0xffffffffu && at + v[j] > target) hit = lane * (SV_SUBS / 32) + j; if (hit == 0xffffffffu) at += v[j]; }
+        for (int j = 0; j < (int)SV_SUBS / 32; ++j) { if (hit == 0xffffffffu && ahead + v[j] > target) hit = lane * (SV_SUBS / 32) + j; if (hit == 0xffffffffu) ahead += v[j]; }
         const uint32_t who = __ffs(__ballot_sync(0xffffffffu, hit != 0xffffffffu)) - 1u;
         const uint32_t b = __shfl_sync(0xffffffffu, hit, who);
-        at = __shfl_sync(0xffffffffu, at, who);
-        uint32_t tie = ranked ? ties_before + s.sub_n[b] : 0;
-        for (uint32_t i = b * sub; i < (b + 1) * sub; i += 32) {
-            const uint64_t w = kept(i + lane, tie), incl = at + warp_scan_u64(w);
+        ahead = __shfl_sync(0xffffffffu, ahead, who);
+        for (uint32_t i0 = b * sub; i0 < (b + 1) * sub; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const uint64_t w = i < n ? value(at[i], i) : 0, incl = ahead + warp_scan_u64(w);
             const uint32_t over = __ballot_sync(0xffffffffu, incl > target);
             if (over) {
-                if (lane == (uint32_t)__ffs(over) - 1u) a.map[od] = (float)(base + i + lane);
+                if (lane == (uint32_t)__ffs(over) - 1u) a.map[od] = (float)(base + i);
                 break;
             }
-            at = __shfl_sync(0xffffffffu, incl, 31);
+            ahead = __shfl_sync(0xffffffffu, incl, 31);
         }
     }
-    cl.sync();                                        // nobody leaves while its shared memory is read
+    together();                                       // nobody leaves while its shared memory is read
+}
+
+template <bool RES>
+static int launch_sample(const SampleArgs& a, uint32_t rows, uint32_t C) {
+    constexpr size_t fixed = (sizeof(SvShared) + 15) / 16 * 16;
+    static bool set = false;
+    if (!set) {
+        if (cudaFuncSetAttribute((const void*)k_sample_vocab<RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + (RES ? SV_RESIDENT * 4 : 0))) != cudaSuccess ||
+            cudaFuncSetAttribute((const void*)k_sample_vocab<RES>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return fail(ADAMAH_ERR_BACKEND, "sample: cannot set the kernel's limits");
+        set = true;
+    }
+    launch_k_cluster(k_sample_vocab<RES>, dim3(rows * C), dim3(SV_T), fixed + (RES ? (size_t)a.chunk * 4 : 0), g.stream, false, C, false, a);
+    count_launch();
+    return check_launch("map_sample");
 }
 
 }  // namespace ab
@@ -510,19 +550,7 @@ extern "C" int map_sample_dev(uint32_t map, uint32_t logits_h, uint32_t rule_h, 
     int lg = 0;
     while ((1ull << lg) < n_vocab) ++lg;
     a.shift = 63 - lg < 50 ? 63 - lg : 50;            // n_vocab weights of at most 2^shift stay below 2^64
-    const bool res = a.chunk <= SV_RESIDENT;
-    void (*k)(const SampleArgs) = res ? k_sample_vocab<true> : k_sample_vocab<false>;
-    const size_t smem = (sizeof(SvShared) + 15) / 16 * 16 + (res ? (size_t)a.chunk * 4 : 0);
-    static bool set[2] = {false, false};
-    if (!set[res]) {
-        if (cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((sizeof(SvShared) + 15) / 16 * 16 + (res ? SV_RESIDENT * 4 : 0))) != cudaSuccess ||
-            cudaFuncSetAttribute((const void*)k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-            return fail(ADAMAH_ERR_BACKEND, "sample: cannot set the kernel's limits");
-        set[res] = true;
-    }
-    launch_k_cluster(k, dim3(n_rows * C), dim3(SV_T), smem, g.stream, false, C, false, a);
-    count_launch();
-    const int rc = check_launch("map_sample");
+    const int rc = a.chunk <= SV_RESIDENT ? launch_sample<true>(a, n_rows, C) : launch_sample<false>(a, n_rows, C);
     end_of_op();
     return rc;
 }
