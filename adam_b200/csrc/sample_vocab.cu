@@ -18,6 +18,7 @@
 #include "common.cuh"
 
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace ab {
 
@@ -26,6 +27,8 @@ namespace cg = cooperative_groups;
 constexpr uint32_t SV_SUBS = 256;                    // stretches of a CTA's share, a sum for each
 constexpr uint32_t SV_RESIDENT = 36864;              // logits that a CTA keeps in shared memory at most
 constexpr uint32_t SV_TABLE = 1024;
+constexpr uint32_t SV_NEAR_BINS = 256;
+enum SvMode { SV_COUNT, SV_NEAR, SV_EXACT };
 constexpr int SV_T = 1024, SV_W = SV_T / 32;
 constexpr uint32_t SV_BINS = 2048, SV_FEW = 2048;    // bins; candidates that one CTA sorts
 
@@ -56,31 +59,29 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v) {      // inclusiv
 }
 
 // Weights as integers.  (max - x) / (T ln 2) = y is formed in two 32-bit words; 2^-y = 2^-k 2^(-i/1024) (1 - s) with the table's
-// entry i, an integer k and s = 1 - 2^-r, |r| <= 2^-11, whose series needs two terms (the third is 7e-12).  s is known to
-// 2^-24 of itself, so a weight to 1e-10 of itself: what is drawn changes with probability 1e-7 or so.  64 rows of 262144, no
-// cuts: 96 us with conversions and the order's keys in the loop, against %PLAIN% us; more with the 64-bit exponential.
+// entry i, an integer k and s = 1 - 2^-r, |r| <= 2^-11, whose series needs two terms (the third is 7e-12).  A weight is known to
+// 5e-10 of itself, so what is drawn changes with probability 1e-7 or so.  What the last unit cuts off is half a unit in the
+// mean: the weights are odd numbers of half units.
 struct SvWeights {
-    const uint64_t* table;                            // 2^62 2^(-i/1024)
+    const uint32_t* table;                            // 2^30 2^(-i/1024)
     float mx, c_hi, c_lo; int shift;
     __device__ __noinline__ uint64_t special(float x) const {        // no finite difference, or nothing left of the weight
-        if (x == mx) return 1ull << shift;
+        if (x == mx) return 1ull << shift | 1u;
         if (!(mx - x > 3.402823466e+38f) || mx > 3.402823466e+38f) return 0;
         const double w = exp2(-(((double)mx - (double)x) * ((double)c_hi + (double)c_lo)));       // the difference of two logits overflows
-        return (uint64_t)__double2ull_rn(w * (double)(1ull << shift));
+        return (uint64_t)(w * (double)(1ull << shift)) | (w > 0.0 ? 1u : 0u);
     }
     __device__ __forceinline__ uint64_t operator()(float x) const {
         constexpr float MAGIC = 12582912.f;            // 1.5 x 2^23: the low bits of a sum with it are the nearest integer
         const float d = mx - x, b = d - mx, d_lo = (mx - (d - b)) + (-x - b);
         const float y = d * c_hi;
-        if (!(y < (float)(shift + 1))) return special(x);            // below half a unit, or not a number
+        if (!(y < (float)shift)) return special(x);    // below a unit, or not a number
         const float t = fmaf(y, (float)SV_TABLE, MAGIC);
         const float r = fmaf(t - MAGIC, -1.f / SV_TABLE, y) + (fmaf(d, c_hi, -y) + fmaf(d, c_lo, d_lo * c_hi));
-        const float z = r * 0.69314718055994530942f, s = fmaf(z * z, -0.5f, z);
+        const float z = r * 0.69314718055994530942f, q = fmaf(z * z, -0.5f, z);
         const uint32_t ti = __float_as_uint(t) & 0x3fffffu;
-        const uint64_t w = table[ti % SV_TABLE];
-        const int cut = __float_as_int(fmaf(s, 4294967296.f, MAGIC)) - __float_as_int(MAGIC);
-        const uint32_t sh = 62 - shift + ti / SV_TABLE;
-        return (w - (uint64_t)((int64_t)(int)(w >> 32) * cut) + (1ull << (sh - 1))) >> sh;
+        const int w = (int)table[ti % SV_TABLE], cut = __float_as_int(fmaf(q, 4294967296.f, MAGIC)) - __float_as_int(MAGIC);
+        return ((uint64_t)(uint32_t)(w - __mulhi(w, cut)) << 33) >> (63 - shift + ti / SV_TABLE) | 1u;
     }
 };
 
@@ -88,13 +89,13 @@ struct SvBins { uint32_t n[SV_BINS], lo[SV_BINS], hi[SV_BINS]; };      // counts
 struct SvShared {
     union { SvBins own; uint64_t list[SV_FEW]; };     // the CTA's histogram; the first CTA's candidates
     union { SvBins all; uint64_t w[SV_FEW]; };        // its share of the cluster's bins, merged; the candidates' weights
-    uint64_t table[SV_TABLE];
-    uint64_t seg_v, pass_v;                           // weight of that share; of what is kept
+    uint32_t table[SV_TABLE];
+    uint64_t seg_v, pass_v, all_v, above_v;           // weight of that share; of what is kept, of all, of the bins ahead of the window
     uint64_t kmin, kmax, least;                       // of the crossing bin; the last that is kept
-    uint32_t n_list, first; float max;
+    uint32_t n_list, first, found; float max;
     uint64_t sub_v[SV_SUBS], wv[SV_W];
     float wmax[SV_W];
-    uint64_t hit_above, hit_v; uint32_t hit_bin, hit_n, hit_count;
+    uint64_t hit_above, hit_v, hit_count; uint32_t hit_bin, hit_n;
     uint64_t peer_v[16];
 };
 
@@ -207,8 +208,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         if (lane == 0) s.max = mx;
     }
     together();
-    mx = -INFINITY;
-    for (uint32_t c = 0; c < C; ++c) mx = fmaxf(mx, *cl.map_shared_rank(&s.max, c));
+    mx = warp_max(lane < C ? *cl.map_shared_rank(&s.max, lane) : -INFINITY);
     if (mx == -INFINITY || !(rule.temperature > 0.f)) {         // nothing to draw, or the first of the largest: the cluster agrees
         if (mx == -INFINITY) { if (lead) a.map[od] = -1.f; }
         else {
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         if (lead && mx != -INFINITY) a.map[od] = (float)s.first;
         return;
     }
-    for (uint32_t i = tid; i < SV_TABLE; i += SV_T) s.table[i] = (uint64_t)__double2ull_rn(exp2(-(double)i / SV_TABLE) * 4611686018427387904.0);
+    for (uint32_t i = tid; i < SV_TABLE; i += SV_T) s.table[i] = __double2uint_rn(exp2(-(double)i / SV_TABLE) * 1073741824.0);
 
     const double c = 1.4426950408889634074 / (double)rule.temperature;
     const float c_hi = (float)c;
@@ -239,20 +239,38 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     bool whole = true;                                // no cut yet: all but -infinity (and NaN)
     auto kept = [&](float x, uint32_t i) { return x > x_t || (x == x_t && !whole && base + i <= i_t); };
 
+    // Histograms: counts, or sums of weights, exact ones or near ones (exact in the first SV_NEAR_BINS, 4 temperatures below the
+    // largest, where single weights matter; counts times the weight in a bin's middle further down).
+    auto clear = [&](SvMode mode) {
+        for (uint32_t b = tid; b < (mode == SV_EXACT ? SV_BINS : SV_NEAR_BINS); b += SV_T) { s.own.lo[b] = 0; s.own.hi[b] = 0; }
+        for (uint32_t b = tid; b < SV_BINS; b += SV_T) s.own.n[b] = 0;
+        __syncthreads();
+    };
+    auto count = [&](uint32_t b, float x, SvMode mode) {
+        atomicAdd(&s.own.n[b], 1u);
+        if (mode == SV_EXACT || (mode == SV_NEAR && b < SV_NEAR_BINS)) {
+            const uint64_t w = weight(x);
+            const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.own.lo[b], lo), hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+            if (hi) atomicAdd(&s.own.hi[b], hi);
+        }
+    };
     // The cluster's histogram: CTA c ends with the bins c * per .. of all, and their totals.
     const uint32_t per = SV_BINS / C;
-    auto merge = [&](bool sums) {
+    auto merge = [&](SvMode mode) {
         together();
         uint64_t tv = 0;
         for (uint32_t b = tid; b < per; b += SV_T) {
+            const uint32_t bin = rank * per + b;
+            const bool sums = mode == SV_EXACT || (mode == SV_NEAR && bin < SV_NEAR_BINS);
             uint32_t cn = 0; uint64_t cv = 0;
 #pragma unroll 4
             for (uint32_t k = 0; k < C; ++k) {
                 const SvBins* h = cl.map_shared_rank(&s.own, k);
-                cn += h->n[rank * per + b];
-                if (sums) cv += (uint64_t)h->lo[rank * per + b] + ((uint64_t)h->hi[rank * per + b] << 32);
+                cn += h->n[bin];
+                if (sums) cv += (uint64_t)h->lo[bin] + ((uint64_t)h->hi[bin] << 32);
             }
-            if (!sums) cv = cn;
+            if (mode == SV_COUNT) cv = cn;
+            else if (!sums) cv = cn * (uint64_t)(exp2f((bin + 0.5f) * (-1.4426950408889634f / 64.f)) * (float)(1ull << a.shift));
             s.all.n[b] = cn; s.all.lo[b] = (uint32_t)cv; s.all.hi[b] = (uint32_t)(cv >> 32);
             tv += cv;
         }
@@ -266,6 +284,21 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         together();
         if (tid < C) s.peer_v[tid] = *cl.map_shared_rank(&s.seg_v, tid);
         __syncthreads();
+    };
+    // A value of every CTA, added up
+    auto add_up = [&](const uint64_t* mine) { return warp_sum_u64(lane < C ? *cl.map_shared_rank(mine, lane) : 0ull); };
+    // How many logits lie in the bins up to `bin`, from the merged histogram
+    auto upto = [&](uint32_t bin) {
+        uint32_t v = 0;
+        for (uint32_t b = tid; b < per; b += SV_T) v += rank * per + b <= bin ? s.all.n[b] : 0u;
+        v = __reduce_add_sync(0xffffffffu, v);
+        if (tid == 0) s.hit_count = 0;
+        __syncthreads();
+        if (lane == 0) atomicAdd((unsigned long long*)&s.hit_count, (unsigned long long)v);
+        together();
+        const uint64_t all = add_up(&s.hit_count);
+        together();
+        return all;
     };
     auto total = [&]() { uint64_t v = 0; for (uint32_t k = 0; k < C; ++k) v += s.peer_v[k]; return v; };
     // exclusive sums over the CTA, and the sum of all
@@ -295,18 +328,6 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
                 above += x;
             }
         __syncthreads();
-    };
-    auto clear = [&](bool sums) {
-        for (uint32_t b = tid; b < SV_BINS; b += SV_T) { s.own.n[b] = 0; if (sums) { s.own.lo[b] = 0; s.own.hi[b] = 0; } }
-        __syncthreads();
-    };
-    auto count = [&](uint32_t b, float x, bool sums) {
-        atomicAdd(&s.own.n[b], 1u);
-        if (sums) {
-            const uint64_t w = weight(x);
-            const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.own.lo[b], lo), hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
-            if (hi) atomicAdd(&s.own.hi[b], hi);
-        }
     };
     auto share = [&](uint64_t all) {                  // top_p of a sum, rounded up, at least one unit
         const uint64_t p = (uint64_t)((double)fmaxf(rule.top_p, 0.f) * 18446744073709551616.0), t = __umul64hi(p, all) + (p * all != 0 ? 1u : 0u);
@@ -360,11 +381,121 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
             ahead += w[j];
         }
     };
+    // Sums over stretches of the row, in index order, of what is kept and weighs enough: all of it, or (window) what lies ahead
+    // of bin b0; the logits of the bins b0 .. b1 then go into the first CTA's list, and all_v and above_v get the weight of all that
+    // is kept and of what lies ahead of b0.
+    const uint32_t sub = max(128u, ((a.chunk + SV_SUBS - 1) / SV_SUBS + 127) & ~127u), n_sub = (n + sub - 1) / sub;
+    auto value = [&](float x, uint32_t i) -> uint64_t {
+        if (!kept(x, i)) return 0;
+        const uint64_t w = weight(x);
+        return w >= least ? w : 0;
+    };
+    auto sweep = [&](auto window, uint32_t b0, uint32_t b1) {
+        uint32_t* const n_list = cl.map_shared_rank(&s.n_list, 0);
+        uint64_t* const list = cl.map_shared_rank(&s.list[0], 0);
+        uint64_t t_all = 0, t_above = 0, sum;
+        auto one = [&](float x, uint32_t i) -> uint64_t {
+            if constexpr (!decltype(window)::value) return value(x, i);
+            else {
+                if (!kept(x, i)) return 0;
+                const uint64_t w = weight(x);
+                const uint32_t bin = bin_of(x);
+                t_all += w;
+                if (bin < b0) { t_above += w; return w >= least ? w : 0; }
+                if (bin <= b1) list[atomicAdd(n_list, 1u)] = sv_key(x, base + i);
+                return 0;
+            }
+        };
+        for (uint32_t b = warp; b < n_sub; b += SV_W) {
+            uint64_t v = 0;
+            const uint32_t end = min(n, (b + 1) * sub);
+            if (RES || aligned) {
+#pragma unroll 2
+                for (uint32_t i = b * sub + 4 * lane; i + 3 < end; i += 128) {
+                    const float4 x = *reinterpret_cast<const float4*>(at + i);
+                    v += one(x.x, i) + one(x.y, i + 1) + one(x.z, i + 2) + one(x.w, i + 3);
+                }
+                if (const uint32_t i = (end & ~3u) + lane; i < end) v += one(at[i], i);
+            } else {
+#pragma unroll 4
+                for (uint32_t i = b * sub + lane; i < end; i += 32) v += one(at[i], i);
+            }
+            v = warp_sum_u64(v);
+            if (lane == 0) s.sub_v[b] = v;
+        }
+        if constexpr (decltype(window)::value) {
+            scan(t_all, sum);
+            if (tid == 0) s.all_v = sum;
+            scan(t_above, sum);
+            if (tid == 0) s.above_v = sum;
+        }
+        __syncthreads();
+    };
+    // The last of the sorted list with which the running sum of its weights (or its count) reaches `rest`; false: it does not.
+    auto last_of_list = [&](uint64_t rest, bool sums) -> bool {
+        uint64_t w[PER], mine = 0, sum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const uint32_t i = tid * PER + j;
+            w[j] = i < s.n_list ? (sums ? weight(sv_value(s.list[i])) : 1ull) : 0;
+            mine += w[j];
+        }
+        uint64_t ahead = scan(mine, sum);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (ahead < rest && rest <= ahead + w[j]) s.least = s.list[tid * PER + j];
+            ahead += w[j];
+        }
+        return rest >= 1 && rest <= sum;
+    };
+    bool swept = false;
+    // The nucleus from counts: they say nearly where its end lies, one pass then has the exact weights and the logits around the
+    // end.  1: the token is drawn, 0: it is cut, -1: the end lies elsewhere, or too many logits around it.
+    auto nucleus = [&]() -> int {
+        clear(SV_NEAR);
+        each([&](float x, uint32_t i) { if (kept(x, i)) count(bin_of(x), x, SV_NEAR); });
+        merge(SV_NEAR);
+        const uint64_t near = total(), target = share(near), slack = near >> 10;
+        cross(target > slack ? target - slack : 1);
+        uint32_t b0 = s.hit_bin;
+        cross(min(near, target + slack));
+        const uint32_t b1 = s.hit_bin;
+        const uint64_t end = upto(b1);
+        bool drawn = whole && end <= SV_FEW;                    // all candidates fit the list
+        if (drawn) b0 = 0;
+        else if (end - (b0 ? upto(b0 - 1) : 0) > SV_FEW) return -1;
+        sweep(std::true_type{}, b0, b1);
+        together();
+        if (rank == 0) {
+            sv_sort(s.list, s.n_list);
+            const uint64_t all = add_up(&s.all_v), above = add_up(&s.above_v), goal = share(all);
+            const bool found = last_of_list(goal > above ? goal - above : 0, true);
+            if (found && drawn) few(all);
+            if (tid < C) *cl.map_shared_rank(&s.found, tid) = found;       // to everyone's own: who has drawn leaves
+            if (tid == 0 && !found) s.n_list = 0;
+        }
+        together();
+        if (!s.found) return -1;
+        if (drawn) return 1;
+        const uint64_t k = *cl.map_shared_rank(&s.least, 0);
+        const uint32_t m = *cl.map_shared_rank(&s.n_list, 0);
+        for (uint32_t j = tid; j < m; j += SV_T) {
+            const uint64_t e = *cl.map_shared_rank(&s.list[j], 0);
+            const uint32_t i = sv_index(e) - base;
+            if (e < k || i >= n) continue;
+            const uint64_t w = weight(sv_value(e));
+            if (w >= least) atomicAdd((unsigned long long*)&s.sub_v[i / sub], (unsigned long long)w);
+        }
+        __syncthreads();
+        x_t = sv_value(k); i_t = sv_index(k); whole = false; swept = true;
+        return 0;
+    };
     // Cuts what is kept to the run that reaches a target: so many logits (sums false), or so much weight.  True: the token is drawn.
     auto cut = [&](bool sums) -> bool {
-        clear(sums);
-        each([&](float x, uint32_t i) { if (kept(x, i)) count(bin_of(x), x, sums); });
-        merge(sums);
+        const SvMode mode = sums ? SV_EXACT : SV_COUNT;
+        clear(mode);
+        each([&](float x, uint32_t i) { if (kept(x, i)) count(bin_of(x), x, mode); });
+        merge(mode);
         const uint64_t all = total();
         if (!sums && all <= rule.top_k) return false;
         const uint64_t target = sums ? share(all) : rule.top_k;
@@ -372,25 +503,10 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint32_t bin = s.hit_bin;
         uint64_t rest = target - s.hit_above;
         uint32_t in = s.hit_n;
-        if (whole) {
-            // how many candidates lie in the bins up to it: where the first CTA can sort them, it does the rest
-            uint64_t upto = s.hit_above + s.hit_v;
-            if (sums) {
-                uint32_t v = 0;
-                for (uint32_t b = tid; b < per; b += SV_T) v += rank * per + b <= bin ? s.all.n[b] : 0u;
-                v = __reduce_add_sync(0xffffffffu, v);
-                if (tid == 0) s.hit_count = 0;
-                __syncthreads();
-                if (lane == 0) atomicAdd(&s.hit_count, v);
-                together();
-                upto = 0;
-                for (uint32_t k = 0; k < C; ++k) upto += *cl.map_shared_rank(&s.hit_count, k);
-            }
-            if (upto <= SV_FEW) {
-                collect([&](float x, uint32_t) { return x > -INFINITY && bin_of(x) <= bin; });
-                if (rank == 0) few(sums ? all : 0);
-                return true;
-            }
+        if (whole && (sums ? upto(bin) : s.hit_above + s.hit_v) <= SV_FEW) {          // the first CTA sorts all candidates and does the rest
+            collect([&](float x, uint32_t) { return x > -INFINITY && bin_of(x) <= bin; });
+            if (rank == 0) few(sums ? all : 0);
+            return true;
         }
         // The crossing bin, then the crossing one of 2048 equal pieces of the range of its logits' keys, and so on until the first
         // CTA can sort what is left (logits that are all equal are told apart by their indices).
@@ -417,9 +533,9 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
                 ranged = true;
             }
             const int sh = max(0, 64 - __clzll(hi - lo) - (11));
-            clear(sums);
-            each([&](float x, uint32_t i) { if (inside(x, i)) count((uint32_t)((hi - sv_key(x, base + i)) >> sh), x, sums); });
-            merge(sums);
+            clear(mode);
+            each([&](float x, uint32_t i) { if (inside(x, i)) count((uint32_t)((hi - sv_key(x, base + i)) >> sh), x, mode); });
+            merge(mode);
             cross(rest);
             in = s.hit_n; rest -= s.hit_above;
             hi -= (uint64_t)s.hit_bin << sh;
@@ -428,19 +544,8 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         }
         collect(inside);
         if (rank == 0) {
-            uint64_t w[PER], mine = 0, sum;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const uint32_t i = tid * PER + j;
-                w[j] = i < s.n_list ? (sums ? weight(sv_value(s.list[i])) : 1ull) : 0;
-                mine += w[j];
-            }
-            uint64_t ahead = scan(mine, sum);
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (ahead < rest && rest <= ahead + w[j]) s.least = s.list[tid * PER + j];
-                ahead += w[j];
-            }
+            last_of_list(rest, sums);
+            __syncthreads();
             if (tid == 0) s.n_list = 0;
         }
         together();
@@ -449,34 +554,18 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         return false;
     };
     if (rule.top_k > 0 && rule.top_k < a.V && cut(false)) return;
-    if (rule.top_p < 1.f && cut(true)) return;
-    __syncthreads();                                  // the table, where nothing was cut
-
-    // ---- the draw: sums of stretches in index order, then the stretch that holds the token ----
-    const uint32_t sub = max(128u, ((a.chunk + SV_SUBS - 1) / SV_SUBS + 127) & ~127u), n_sub = (n + sub - 1) / sub;
-    auto value = [&](float x, uint32_t i) -> uint64_t {
-        if (!kept(x, i)) return 0;
-        const uint64_t w = weight(x);
-        return w >= least ? w : 0;
-    };
-    for (uint32_t b = warp; b < n_sub; b += SV_W) {
-        uint64_t v = 0;
-        const uint32_t end = min(n, (b + 1) * sub);
-        if (RES || aligned) {
-#pragma unroll 2
-            for (uint32_t i = b * sub + 4 * lane; i + 3 < end; i += 128) {
-                const float4 x = *reinterpret_cast<const float4*>(at + i);
-                v += value(x.x, i) + value(x.y, i + 1) + value(x.z, i + 2) + value(x.w, i + 3);
-            }
-            if (const uint32_t i = (end & ~3u) + lane; i < end) v += value(at[i], i);
-        } else {
-#pragma unroll 4
-            for (uint32_t i = b * sub + lane; i < end; i += 32) v += value(at[i], i);
-        }
-        v = warp_sum_u64(v);
-        if (lane == 0) s.sub_v[b] = v;
+    if (rule.top_p < 1.f) {
+        // a weight for every logit twice, here and in the draw, costs less than nucleus() where a CTA has few of them
+        // (a row of 32003 on eight CTAs 17 against 25 us; 64 rows of 262144 on two each 153 against 133)
+        const int done = RES ? -1 : nucleus();
+        if (done > 0 || (done < 0 && cut(true))) return;
     }
-    __syncthreads();
+
+    // ---- the draw: the stretch that holds the token, then the token ----
+    if (!swept) {
+        __syncthreads();                              // the table, where nothing was cut
+        sweep(std::false_type{}, 0, 0);
+    }
     if (warp == 0) {
         uint64_t v = 0;
         for (uint32_t b = lane; b < n_sub; b += 32) v += s.sub_v[b];
@@ -484,8 +573,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         if (lane == 0) s.pass_v = v;
     }
     together();
-    uint64_t before = 0, all = 0;
-    for (uint32_t k = 0; k < C; ++k) { const uint64_t v = *cl.map_shared_rank(&s.pass_v, k); before += k < rank ? v : 0; all += v; }
+    const uint64_t share_v = lane < C ? *cl.map_shared_rank(&s.pass_v, lane) : 0, before = warp_sum_u64(lane < rank ? share_v : 0), all = warp_sum_u64(share_v);
     const uint64_t target = __umul64hi((uint64_t)((double)u * 18446744073709551616.0), all);     // the running sum to be exceeded
     if (before <= target && target < before + s.pass_v && warp == 0) {
         uint64_t v[SV_SUBS / 32], mine = 0;                        // lane l: stretches 8 l ..
