@@ -19,10 +19,285 @@
 
 namespace ab {
 
+constexpr float FLT_TOP = 3.402823466e+38f;
+
+// 16-byte words of 16-bit rows, so that eight neighbouring rows of one column lie in different banks
+template <int HD>
+__device__ __forceinline__ int swz(int r, int ch) { return HD >= 64 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3); }
+
+// A query row into shared memory by a warp: two fp16 planes (`plane` halves apart) of the row times a power of two, whose inverse
+// comes back, or floats.
+template <typename T, int HD, int LD>
+__device__ __forceinline__ float put_query(const AttnArgs& a, const AttnRow& row, uint8_t* sq, int r, int plane) {
+    const int lane = threadIdx.x & 31;
+    float v[HD / 32], most = 0.f, up = 1.f, down = 1.f;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) { v[j] = row.pos >= 0 ? a.act[row.q + lane + 32 * j] : 0.f; most = fmaxf(most, fabsf(v[j])); }
+    if (sizeof(T) == 2) row_scale(warp_max(most), up, down);
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+        const int d = lane + 32 * j;
+        if constexpr (sizeof(T) == 2) {
+            const float y = v[j] * up;
+            const __half hi = __float2half_rn(y);
+            __half* p = reinterpret_cast<__half*>(sq) + r * HD + swz<HD>(r, d >> 3) * 8 + (d & 7);
+            p[0] = hi; p[plane] = __float2half_rn(y - __half2float(hi));
+        } else reinterpret_cast<float*>(sq)[r * LD + d] = v[j];
+    }
+    return down;
+}
+// Scores of 16 rows (r0 ..) and 8 NT positions (p0 ..): s[n][e] is row r0 + g + 8 (e >> 1), position p0 + 8 n + 2 q4 + (e & 1).
+template <int HD, int NT>
+__device__ __forceinline__ void scores_h(float (&s)[NT][4], uint32_t q_s, int plane, int r0, uint32_t k_s, int p0) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < HD / 16; ++k) {
+        uint32_t qh[4], ql[4];
+        const int qr = r0 + (lane & 15), qc = 2 * k + (lane >> 4);
+        const uint32_t qo = q_s + (uint32_t)(qr * HD + swz<HD>(qr, qc) * 8) * 2u;
+        at_ldsm(qo, qh);
+        at_ldsm(qo + plane * 2, ql);
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n) {
+            uint32_t b[4];
+            const int kr = p0 + n * 16 + (lane >> 4) * 8 + (lane & 7), kc = 2 * k + ((lane >> 3) & 1);
+            at_ldsm(k_s + (uint32_t)(kr * HD + swz<HD>(kr, kc) * 8) * 2u, b);
+            at_mma_h(s[2 * n], ql, b[0], b[1]); at_mma_h(s[2 * n + 1], ql, b[2], b[3]);
+            at_mma_h(s[2 * n], qh, b[0], b[1]); at_mma_h(s[2 * n + 1], qh, b[2], b[3]);
+        }
+    }
+}
+// The same over floats; sums leave the tensor core every 64 dims (96 steps of a head of 256 made 3e-6 of the result)
+template <int HD, int LD, int NT>
+__device__ __forceinline__ void scores_f(float (&s)[NT][4], const float* q, int r0, const float* k_rows, int p0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+    constexpr int PART = HD < 64 ? HD : 64;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll 1
+    for (int k0 = 0; k0 < HD; k0 += PART) {
+        float acc[NT][4] = {};
+#pragma unroll 4
+        for (int k = k0; k < k0 + PART; k += 8) {
+            const float* qp = q + (r0 + g) * LD + k + q4;
+            uint32_t ah[4], al[4];
+            at_split_t(qp[0], ah[0], al[0]); at_split_t(qp[8 * LD], ah[1], al[1]);
+            at_split_t(qp[4], ah[2], al[2]); at_split_t(qp[8 * LD + 4], ah[3], al[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float* kp = k_rows + (p0 + n * 8 + g) * LD + k + q4;
+                uint32_t b0h, b0l, b1h, b1l;
+                at_split_t(kp[0], b0h, b0l); at_split_t(kp[4], b1h, b1l);
+                at_mma_t(acc[n], al, b0h, b1h); at_mma_t(acc[n], ah, b0l, b1l); at_mma_t(acc[n], ah, b0h, b1h);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] += acc[n][e];
+    }
+}
+// Scores to weights: running maximum and sum of each row over its quad of lanes; alpha: the factor of what was summed before.
+template <int NT>
+__device__ __forceinline__ void weights(float (&s)[NT][4], const AttnArgs& a, bool all, const int32_t (&pos)[2], const float (&scl)[2], int32_t p0, float (&m)[2],
+                                        float (&l)[2], float (&alpha)[2]) {
+    const int q4 = threadIdx.x & 3;
+    const float rcap = a.cap > 0.f ? __frcp_rn(a.cap) : 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                float y = s[n][e] * scl[h];
+                if (a.cap > 0.f) y = a.cap * at_tanh(y * rcap);
+                if (!all && !row_sees(a, pos[h], p0 + 8 * n + 2 * q4 + (e & 1))) y = -INFINITY;
+                s[n][e] = y;
+                mx = max_nan(mx, y);
+            }
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = max_nan(m[h], mx), ref = mn == -INFINITY ? 0.f : mn;
+        alpha[h] = expf(m[h] - ref);
+        m[h] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 2 * h; e < 2 * h + 2; ++e) { s[n][e] = expf(s[n][e] - ref); sum += s[n][e]; }
+        l[h] = fmaf(l[h], alpha[h], sum);
+    }
+}
+// o = o alpha + weights x values of the positions p0 .. p0 + 8 NT - 1 (fp16: times 256, which keeps the low terms clear of the
+// subnormals)
+template <int HD, int NT>
+__device__ __forceinline__ void values_h(float (&o)[HD / 8][4], const float (&s)[NT][4], const float (&alpha)[2], uint32_t v_s, int p0) {
+    const int lane = threadIdx.x & 31;
+    uint32_t ph[NT / 2][4], pl[NT / 2][4];
+#pragma unroll
+    for (int k = 0; k < NT / 2; ++k)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            const float* p = &s[2 * k + (f >> 1)][2 * (f & 1)];
+            at_split_h(p[0] * 256.f, p[1] * 256.f, ph[k][f], pl[k][f]);
+        }
+    constexpr int DC = HD == 256 && NT > 2 ? 32 : HD >= 64 ? 64 : HD;     // dims per round: what the registers beside `o` allow
+#pragma unroll
+    for (int d0 = 0; d0 < HD; d0 += DC) {
+        float acc[DC / 8][4] = {};
+#pragma unroll
+        for (int k = 0; k < NT / 2; ++k)
+#pragma unroll
+            for (int n = 0; n < DC / 16; ++n) {
+                uint32_t b[4];
+                const int vr = p0 + k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), vc = d0 / 8 + 2 * n + (lane >> 4);
+                at_ldsm_t(v_s + (uint32_t)(vr * HD + swz<HD>(vr, vc) * 8) * 2u, b);
+                at_mma_h(acc[2 * n], pl[k], b[0], b[1]); at_mma_h(acc[2 * n + 1], pl[k], b[2], b[3]);
+                at_mma_h(acc[2 * n], ph[k], b[0], b[1]); at_mma_h(acc[2 * n + 1], ph[k], b[2], b[3]);
+            }
+#pragma unroll
+        for (int j = 0; j < DC / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d0 / 8 + j][e] = fmaf(o[d0 / 8 + j][e], alpha[e >> 1], acc[j][e]);
+    }
+}
+// The order of the positions inside a step of 8 is free: slots t and t + 4 are positions 2 t and 2 t + 1, which is how the scores lie
+// in the registers.
+template <int HD, int LD, int NT>
+__device__ __forceinline__ void values_f(float (&o)[HD / 8][4], const float (&s)[NT][4], const float (&alpha)[2], const float* v_rows, int p0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+    uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        at_split_t(s[n][0], ph[n][0], pl[n][0]); at_split_t(s[n][2], ph[n][1], pl[n][1]);
+        at_split_t(s[n][1], ph[n][2], pl[n][2]); at_split_t(s[n][3], ph[n][3], pl[n][3]);
+    }
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) {
+        float acc[4] = {};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float* vp = v_rows + (p0 + n * 8 + 2 * q4) * LD + j * 8 + g;
+            uint32_t b0h, b0l, b1h, b1l;
+            at_split_t(vp[0], b0h, b0l); at_split_t(vp[LD], b1h, b1l);
+            at_mma_t(acc, pl[n], b0h, b1h); at_mma_t(acc, ph[n], b0l, b1l); at_mma_t(acc, ph[n], b0h, b1h);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], alpha[e >> 1], acc[e]);
+    }
+}
+
+// What is left at the end: PLANES sets of warps hold sums over different positions of the same ROWS rows (set k's warps the row
+// groups r0 = 0, 16, ..).  They meet in shared memory (`merge`), then the CTAs that share the tile in global memory, the last one
+// to arrive adds up in their order and writes the results; rows that are not finite are done once more, by themselves.
+template <int ROWS, int PLANES>
+struct End { float m[PLANES][ROWS], l[PLANES][ROWS]; uint32_t bad[(ROWS + 31) / 32], ticket; };
+
+template <typename T, int HD, int ROWS, int PLANES>
+__device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
+                                       int plane, int r0, const float (&o)[HD / 8][4], const float (&m)[2], float (&l)[2], float* merge, End<ROWS, PLANES>& end) {
+    constexpr int LM = HD + 4;
+    constexpr float UNIT = sizeof(T) == 2 ? 1.f / 256.f : 1.f;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (q4 == 0) { end.m[plane][r0 + g + 8 * h] = m[h]; end.l[plane][r0 + g + 8 * h] = l[h]; }
+    }
+    if (tid < (ROWS + 31) / 32) end.bad[tid] = 0;
+    __syncthreads();                                     // (and nobody reads what `merge` lies on any more)
+    float best[2], sum[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = r0 + g + 8 * h;
+        best[h] = -INFINITY; sum[h] = 0.f;
+#pragma unroll
+        for (int w = 0; w < PLANES; ++w) best[h] = max_nan(best[h], end.m[w][r]);
+        const float ref = best[h] == -INFINITY ? 0.f : best[h];
+#pragma unroll
+        for (int w = 0; w < PLANES; ++w) sum[h] += end.l[w][r] * expf(end.m[w][r] - ref);
+        const float f = expf(m[h] - ref) * UNIT;
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j)
+            *reinterpret_cast<float2*>(merge + (plane * ROWS + r) * LM + 8 * j + 2 * q4) = make_float2(o[j][2 * h] * f, o[j][2 * h + 1] * f);
+    }
+    __syncthreads();
+    if (plane == 0 && q4 == 0)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { end.m[0][r0 + g + 8 * h] = best[h]; end.l[0][r0 + g + 8 * h] = sum[h]; }
+    __syncthreads();
+    const uint32_t live = min((uint32_t)ROWS, x.n * a.group - x.first);
+    auto value = [&](uint32_t r, uint32_t d) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < PLANES; ++w) v += merge[(w * ROWS + r) * LM + d];
+        return v;
+    };
+    if (sharers > 1) {
+        const size_t tile = (size_t)t * a.geo.n_kv + kvh, step = (size_t)ROWS * (HD + 2);
+        float* mine = a.part + (tile * a.splits + split) * step;
+        for (uint32_t i = tid; i < live * HD; i += nt) mine[ROWS * 2 + i] = value(i / HD, i % HD);
+        if (tid < (int)live) { mine[2 * tid] = end.m[0][tid]; mine[2 * tid + 1] = end.l[0][tid]; }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) end.ticket = atomicInc(a.tickets + tile, sharers - 1);
+        __syncthreads();
+        if (end.ticket != sharers - 1) return;
+        __threadfence();
+        const float* all = a.part + tile * a.splits * step;
+        for (uint32_t r = tid; r < live; r += nt) {
+            float b = -INFINITY, z = 0.f;
+            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, __ldcg(all + k * step + 2 * r));
+            const float ref = b == -INFINITY ? 0.f : b;
+            for (uint32_t k = 0; k < sharers; ++k) z += __ldcg(all + k * step + 2 * r + 1) * expf(__ldcg(all + k * step + 2 * r) - ref);
+            end.m[0][r] = ref; end.l[0][r] = z;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < live * HD; i += nt) {
+            const uint32_t r = i / HD;
+            float v = 0.f;
+#pragma unroll 8
+            for (uint32_t k = 0; k < sharers; ++k) v = fmaf(__ldcg(all + k * step + ROWS * 2 + i), expf(__ldcg(all + k * step + 2 * r) - end.m[0][r]), v);
+            merge[r * LM + i % HD] = v;
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < live * HD; i += nt) {
+        const uint32_t r = i / HD, d = i % HD;
+        const float v = (sharers > 1 ? merge[r * LM + d] : value(r, d)) / end.l[0][r];
+        if (rows[r].pos < 0) continue;
+        if (!(fabsf(v) <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
+        merge[r * LM + d] = v;
+    }
+    __syncthreads();
+    auto bad = [&](uint32_t r) { return end.bad[r >> 5] >> (r & 31) & 1u; };
+    for (uint32_t i = tid; i < live * HD; i += nt) {
+        const uint32_t r = i / HD, d = i % HD;
+        if (rows[r].pos >= 0 && !bad(r)) a.act[rows[r].o + d] = merge[r * LM + d];
+    }
+    for (uint32_t r = tid >> 5; r < live; r += nt >> 5)
+        if (bad(r)) attend_row<T, HD>(a, x, rows[r], kvh);
+}
+// This CTA's chunks of the tile; false: it has none
+__device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, uint32_t split, uint32_t& sharers, uint32_t& c0, uint32_t& c1) {
+    const uint32_t each = max((x.chunks + a.splits - 1) / a.splits, a.least);
+    sharers = (x.chunks + each - 1) / each;
+    c0 = split * each; c1 = min(x.chunks, c0 + each);
+    return split < sharers;
+}
+
 // ---- few rows: 16 per tile -------------------------------------------------------------------------------------------
 // Every warp has chunks of 16 positions of its own (chunk w, w + W, ..), the next ones under way in STAGES slots of
-// shared memory, and its own running maxima, sums and outputs; nothing in the loop waits for another warp.  The warps, then the
-// CTAs that share the tile, merge at the end.  Bound by HBM: the tensor cores are busy for a few percent.
+// shared memory, and its own running maxima, sums and outputs; nothing in the loop waits for another warp.  Bound by HBM: the tensor
+// cores are busy for a few percent.
 template <typename T, int HD>
 struct Few {
     static constexpr int ROWS = 16, CB = 16, ROW_BYTES = HD * (int)sizeof(T);
@@ -35,10 +310,6 @@ struct Few {
     static_assert(SMEM <= 225 * 1024, "shared memory");
 };
 
-// 16-byte words of 16-bit rows, so that eight neighbouring rows of one column lie in different banks
-template <int HD>
-__device__ __forceinline__ int swz(int r, int ch) { return HD >= 64 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3); }
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_constant__ AttnArgs a) {
     using F = Few<T, HD>;
@@ -46,22 +317,18 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
     constexpr bool H = sizeof(T) == 2;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ AttnRow s_row[ROWS];
-    __shared__ float s_unit[ROWS], s_m[W][ROWS], s_l[W][ROWS];
+    __shared__ float s_unit[ROWS];
     __shared__ uint32_t s_scratch[W + 2];
-    __shared__ uint32_t s_bad;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+    __shared__ End<ROWS, W> s_end;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = blockIdx.x / a.splits;
     AttnTile x;
     if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_scratch)) return;
-    // this CTA's chunks
-    const uint32_t each = max((x.chunks + a.splits - 1) / a.splits, a.least), sharers = (x.chunks + each - 1) / each;
-    if (split >= sharers) return;
-    const uint32_t c0 = split * each, c1 = min(x.chunks, c0 + each);
-    if (tid == 0) s_bad = 0;
+    uint32_t sharers, c0, c1;
+    if (!share_out(a, x, split, sharers, c0, c1)) return;
 
-    uint8_t* const sq = sm;                              // the queries
     uint8_t* const ring = sm + F::Q_BYTES + warp * STAGES * F::SLOT;
-    const uint32_t ring_s = at_smem(ring);
+    const uint32_t ring_s = at_smem(ring), q_s = at_smem(sm);
     const T* const pool = reinterpret_cast<const T*>(a.pool);
     const size_t v_off = (size_t)a.geo.n_kv * a.geo.page * HD;
     // Chunks of this warp: c0 + warp, + W, ...  Lane l knows where position l % 16 of the next one to be asked for lies.
@@ -87,29 +354,12 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
     };
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; ++i) request(i);
-    // queries: fp16 terms of the row times a power of two, or floats; a warp takes every fourth row
     for (int r = warp; r < ROWS; r += W) {
-        const AttnRow row = s_row[r];
-        float v[HD / 32], most = 0.f;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) { v[j] = row.pos >= 0 ? a.act[row.q + lane + 32 * j] : 0.f; most = fmaxf(most, fabsf(v[j])); }
-        float up = 1.f, down = 1.f;
-        if (H) row_scale(warp_max(most), up, down);
-        if (lane == 0) s_unit[r] = down;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-            const int d = lane + 32 * j;
-            if constexpr (H) {
-                const float y = v[j] * up;
-                const __half hi = __float2half_rn(y);
-                __half* p = reinterpret_cast<__half*>(sq) + r * HD + swz<HD>(r, d >> 3) * 8 + (d & 7);
-                p[0] = hi; p[ROWS * HD] = __float2half_rn(y - __half2float(hi));
-            } else reinterpret_cast<float*>(sq)[r * LD + d] = v[j];
-        }
+        const float unit = put_query<T, HD, LD>(a, s_row[r], sm, r, ROWS * HD);
+        if (lane == 0) s_unit[r] = unit;
     }
     __syncthreads();
 
-    const uint32_t sq_s = at_smem(sq);
     const int32_t pos[2] = {s_row[g].pos, s_row[g + 8].pos};
     const float scl[2] = {s_unit[g] * a.scale, s_unit[g + 8] * a.scale};
     float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -117,230 +367,154 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
     for (int j = 0; j < HD / 8; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-
     int slot = 0;
 #pragma unroll 1
     for (uint32_t c = c0 + warp; c < c1; c += W) {
         at_wait<STAGES - 2>();
         __syncwarp();
-        const uint32_t k_s = ring_s + slot * F::SLOT, v_s = k_s + F::SLOT / 2;
-        const float *kf = reinterpret_cast<const float*>(ring + slot * F::SLOT), *vf = kf + CB * LD;
+        const uint32_t k_s = ring_s + slot * F::SLOT;
+        const float* kf = reinterpret_cast<const float*>(ring + slot * F::SLOT);
         request(slot ? slot - 1 : STAGES - 1);           // the slot that the chunk before this one has left
         const int32_t p0 = chunk_at<CB>(x, c);
-        float s[2][4] = {};                              // scores: positions p0 + 8 n + 2 q4 + (e & 1), rows g + 8 (e >> 1)
-        if constexpr (H) {
-#pragma unroll 4
-            for (int k = 0; k < HD / 16; ++k) {
-                uint32_t qh[4], ql[4], b[4];
-                const int qr = lane & 15, qc = 2 * k + (lane >> 4), kr = (lane >> 4) * 8 + (lane & 7), kc = 2 * k + ((lane >> 3) & 1);
-                const uint32_t qo = (uint32_t)(qr * HD + swz<HD>(qr, qc) * 8) * 2u;
-                at_ldsm(sq_s + qo, qh);
-                at_ldsm(sq_s + ROWS * HD * 2 + qo, ql);
-                at_ldsm(k_s + (uint32_t)(kr * HD + swz<HD>(kr, kc) * 8) * 2u, b);
-                at_mma_h(s[0], ql, b[0], b[1]); at_mma_h(s[1], ql, b[2], b[3]);
-                at_mma_h(s[0], qh, b[0], b[1]); at_mma_h(s[1], qh, b[2], b[3]);
-            }
-        } else {
-#pragma unroll 4
-            for (int k = 0; k < HD; k += 8) {
-                const float* qp = reinterpret_cast<const float*>(sq) + g * LD + k + q4;
-                uint32_t ah[4], al[4];
-                at_split_t(qp[0], ah[0], al[0]); at_split_t(qp[8 * LD], ah[1], al[1]);
-                at_split_t(qp[4], ah[2], al[2]); at_split_t(qp[8 * LD + 4], ah[3], al[3]);
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float* kp = kf + (n * 8 + g) * LD + k + q4;
-                    uint32_t b0h, b0l, b1h, b1l;
-                    at_split_t(kp[0], b0h, b0l); at_split_t(kp[4], b1h, b1l);
-                    at_mma_t(s[n], al, b0h, b1h); at_mma_t(s[n], ah, b0l, b1l); at_mma_t(s[n], ah, b0h, b1h);
-                }
-            }
-        }
-        // weights: running maximum and sum of each row over its quad of lanes
-        const bool all = tile_sees(a, x, p0, CB);
-        float alpha[2];
-        const float rcap = a.cap > 0.f ? __frcp_rn(a.cap) : 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 2 * h; e < 2 * h + 2; ++e) {
-                    float y = s[n][e] * scl[h];
-                    if (a.cap > 0.f) y = a.cap * at_tanh(y * rcap);
-                    if (!all && !row_sees(a, pos[h], p0 + 8 * n + 2 * q4 + (e & 1))) y = -INFINITY;
-                    s[n][e] = y;
-                    mx = max_nan(mx, y);
-                }
-            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = max_nan(m[h], mx), ref = mn == -INFINITY ? 0.f : mn;
-            alpha[h] = expf(m[h] - ref);
-            m[h] = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 2 * h; e < 2 * h + 2; ++e) { s[n][e] = expf(s[n][e] - ref); sum += s[n][e]; }
-            l[h] = fmaf(l[h], alpha[h], sum);
-        }
-        if constexpr (H) {
-            uint32_t ph[4], pl[4];                       // times 256: the low terms stay clear of the fp16 subnormals
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                const float* p = &s[f >> 1][2 * (f & 1)];
-                at_split_h(p[0] * 256.f, p[1] * 256.f, ph[f], pl[f]);
-            }
-            constexpr int DC = HD >= 64 ? 64 : HD;
-#pragma unroll
-            for (int d0 = 0; d0 < HD; d0 += DC) {
-                float acc[DC / 8][4] = {};
-#pragma unroll
-                for (int n = 0; n < DC / 16; ++n) {
-                    uint32_t b[4];
-                    const int vr = ((lane >> 3) & 1) * 8 + (lane & 7), vc = d0 / 8 + 2 * n + (lane >> 4);
-                    at_ldsm_t(v_s + (uint32_t)(vr * HD + swz<HD>(vr, vc) * 8) * 2u, b);
-                    at_mma_h(acc[2 * n], pl, b[0], b[1]); at_mma_h(acc[2 * n + 1], pl, b[2], b[3]);
-                    at_mma_h(acc[2 * n], ph, b[0], b[1]); at_mma_h(acc[2 * n + 1], ph, b[2], b[3]);
-                }
-#pragma unroll
-                for (int j = 0; j < DC / 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[d0 / 8 + j][e] = fmaf(o[d0 / 8 + j][e], alpha[e >> 1], acc[j][e]);
-            }
-        } else {
-            // the order of the positions inside a step of 8 is free: slots t and t + 4 are positions 2 t and 2 t + 1, which is
-            // how the scores lie in the registers
-            uint32_t ph[2][4], pl[2][4];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                at_split_t(s[n][0], ph[n][0], pl[n][0]); at_split_t(s[n][2], ph[n][1], pl[n][1]);
-                at_split_t(s[n][1], ph[n][2], pl[n][2]); at_split_t(s[n][3], ph[n][3], pl[n][3]);
-            }
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j) {
-                float acc[4] = {};
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float* vp = vf + (n * 8 + 2 * q4) * LD + j * 8 + g;
-                    uint32_t b0h, b0l, b1h, b1l;
-                    at_split_t(vp[0], b0h, b0l); at_split_t(vp[LD], b1h, b1l);
-                    at_mma_t(acc, pl[n], b0h, b1h); at_mma_t(acc, ph[n], b0l, b1l); at_mma_t(acc, ph[n], b0h, b1h);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], alpha[e >> 1], acc[e]);
-            }
-        }
+        float s[2][4], alpha[2];
+        if constexpr (H) scores_h<HD, 2>(s, q_s, ROWS * HD, 0, k_s, 0);
+        else scores_f<HD, LD, 2>(s, reinterpret_cast<const float*>(sm), 0, kf, 0);
+        weights<2>(s, a, tile_sees(a, x, p0, CB), pos, scl, p0, m, l, alpha);
+        if constexpr (H) values_h<HD, 2>(o, s, alpha, k_s + F::SLOT / 2, 0);
+        else values_f<HD, LD, 2>(o, s, alpha, kf + CB * LD, 0);
         slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     at_wait<0>();
-
-    // ---- the warps' results ----
-    constexpr float UNIT = H ? 1.f / 256.f : 1.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if (q4 == 0) { s_m[warp][g + 8 * h] = m[h]; s_l[warp][g + 8 * h] = l[h]; }
-    }
-    __syncthreads();
-    float* const merge = reinterpret_cast<float*>(sm + F::Q_BYTES);       // [warp][row][HD + 4]
-    float best[2], sum[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        best[h] = -INFINITY; sum[h] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) best[h] = max_nan(best[h], s_m[w][g + 8 * h]);
-        const float ref = best[h] == -INFINITY ? 0.f : best[h];
-#pragma unroll
-        for (int w = 0; w < W; ++w) sum[h] += s_l[w][g + 8 * h] * expf(s_m[w][g + 8 * h] - ref);
-        const float f = expf(m[h] - ref) * UNIT;
-#pragma unroll
-        for (int j = 0; j < HD / 8; ++j)
-            *reinterpret_cast<float2*>(merge + (warp * ROWS + g + 8 * h) * (HD + 4) + 8 * j + 2 * q4) = make_float2(o[j][2 * h] * f, o[j][2 * h + 1] * f);
-    }
-    __syncthreads();
-    if (warp == 0 && q4 == 0)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) { s_m[0][g + 8 * h] = best[h]; s_l[0][g + 8 * h] = sum[h]; }
-    __syncthreads();
-    const uint32_t live = min((uint32_t)ROWS, x.n * a.group - x.first);
-    auto value = [&](uint32_t r, uint32_t d) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) v += merge[(w * ROWS + r) * (HD + 4) + d];
-        return v;
-    };
-    if (sharers > 1) {
-        // a partial result per CTA; the last one to arrive adds them up in their order
-        const size_t tile = (size_t)t * a.geo.n_kv + kvh;
-        float* mine = a.part + (tile * a.splits + split) * ROWS * (HD + 2);
-        for (uint32_t i = tid; i < live * HD; i += W * 32) mine[ROWS * 2 + i] = value(i / HD, i % HD);
-        if (tid < (int)live) { mine[2 * tid] = s_m[0][tid]; mine[2 * tid + 1] = s_l[0][tid]; }
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) s_scratch[0] = atomicInc(a.tickets + tile, sharers - 1);
-        __syncthreads();
-        if (s_scratch[0] != sharers - 1) return;
-        __threadfence();
-        const float* all = a.part + tile * a.splits * ROWS * (HD + 2);
-        const size_t step = (size_t)ROWS * (HD + 2);
-        if (tid < (int)live) {
-            float b = -INFINITY, z = 0.f;
-            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, __ldcg(all + k * step + 2 * tid));
-            const float ref = b == -INFINITY ? 0.f : b;
-            for (uint32_t k = 0; k < sharers; ++k) z += __ldcg(all + k * step + 2 * tid + 1) * expf(__ldcg(all + k * step + 2 * tid) - ref);
-            s_m[0][tid] = ref; s_l[0][tid] = z;
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < live * HD; i += W * 32) {
-            const uint32_t r = i / HD;
-            float v = 0.f;
-#pragma unroll 8
-            for (uint32_t k = 0; k < sharers; ++k) v = fmaf(__ldcg(all + k * step + ROWS * 2 + i), expf(__ldcg(all + k * step + 2 * r) - s_m[0][r]), v);
-            merge[r * (HD + 4) + i % HD] = v;
-        }
-        __syncthreads();
-    }
-    // ---- out; rows that are not finite once more, by themselves ----
-    for (uint32_t i = tid; i < live * HD; i += W * 32) {
-        const uint32_t r = i / HD, d = i % HD;
-        const float v = (sharers > 1 ? merge[r * (HD + 4) + d] : value(r, d)) / s_l[0][r];
-        if (s_row[r].pos < 0) continue;
-        if (!(fabsf(v) <= 3.402823466e+38f)) atomicOr(&s_bad, 1u << r);
-        merge[r * (HD + 4) + d] = v;
-    }
-    __syncthreads();
-    const uint32_t bad = s_bad;
-    for (uint32_t i = tid; i < live * HD; i += W * 32) {
-        const uint32_t r = i / HD, d = i % HD;
-        if (s_row[r].pos >= 0 && !(bad >> r & 1u)) a.act[s_row[r].o + d] = merge[r * (HD + 4) + d];
-    }
-    if (bad)
-        for (uint32_t r = warp; r < live; r += W)
-            if (bad >> r & 1u) attend_row<T, HD>(a, x, s_row[r], kvh);
+    finish<T, HD, ROWS, W>(a, x, s_row, t, kvh, split, sharers, warp, 0, o, m, l, reinterpret_cast<float*>(sm + F::Q_BYTES), s_end);
 }
 
-template <typename T, int HD>
-static int launch_few(AttnArgs& a, uint32_t tiles) {
-    using F = Few<T, HD>;
-    static bool set = false;
+// ---- many rows: 32 to 128 per tile -----------------------------------------------------------------------------------
+// RG groups of 16 rows, KH warps to a group, each with its share of every chunk's positions; two chunks of keys and values in
+// shared memory for all of them.
+template <typename T, int HD, int RG, int KH>
+struct Many {
+    static constexpr int ROWS = RG * 16, CB = sizeof(T) == 2 ? 64 : 32, LD = sizeof(T) == 2 ? HD : HD + 4;
+    static constexpr int PART = CB * LD * (int)sizeof(T);                         // keys, or values, of a chunk
+    static constexpr int Q_BYTES = ROWS * LD * 4, MERGE = KH * ROWS * (HD + 4) * 4;
+    static constexpr int SMEM = Q_BYTES + 4 * PART > MERGE ? Q_BYTES + 4 * PART : MERGE;
+    static_assert(SMEM <= 225 * 1024, "shared memory");
+};
+
+template <typename T, int HD, int RG, int KH>
+__global__ void __launch_bounds__(RG * KH * 32) k_attn_many(const __grid_constant__ AttnArgs a) {
+    using F = Many<T, HD, RG, KH>;
+    constexpr int ROWS = F::ROWS, CB = F::CB, LD = F::LD, NT = CB / KH / 8, THREADS = RG * KH * 32;
+    constexpr bool H = sizeof(T) == 2;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ AttnRow s_row[ROWS];
+    __shared__ float s_unit[ROWS];
+    __shared__ uint32_t s_scratch[RG * KH + 2];
+    __shared__ int64_t s_where[2][CB];
+    __shared__ End<ROWS, KH> s_end;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rg = warp % RG, kh = warp / RG, r0 = rg * 16, g = lane >> 2;
+    const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = blockIdx.x / a.splits;
+    AttnTile x;
+    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_scratch)) return;
+    uint32_t sharers, c0, c1;
+    if (!share_out(a, x, split, sharers, c0, c1)) return;
+    uint8_t* const tiles = sm + F::Q_BYTES;              // chunk c: keys at (c & 1) * 2 PART, values behind them
+    const uint32_t tiles_s = at_smem(tiles), q_s = at_smem(sm);
+    const T* const pool = reinterpret_cast<const T*>(a.pool);
+    const size_t v_off = (size_t)a.geo.n_kv * a.geo.page * HD;
+    auto locate = [&](uint32_t c) { if (tid < CB) s_where[c & 1][tid] = c < c1 ? tile_position(a, x, kvh, chunk_at<CB>(x, c) + tid) : -1; };
+    auto request = [&](uint32_t c) {                     // c < c1: chunk c, whose positions are located
+        constexpr int WPR = HD * (int)sizeof(T) / 16;
+        if (c < c1) {
+            const uint32_t base = tiles_s + (c & 1) * 2 * F::PART;
+#pragma unroll 4
+            for (int w = tid; w < CB * WPR; w += THREADS) {
+                const int r = w / WPR, ch = w % WPR;
+                const int64_t at = s_where[c & 1][r];
+                const T* src = pool + (at < 0 ? 0 : at) + ch * (16 / sizeof(T));
+                const uint32_t dst = base + (H ? (uint32_t)(r * HD + swz<HD>(r, ch) * 8) * 2u : (uint32_t)(r * LD + ch * 4) * 4u);
+                at_cp16(dst, src, at >= 0);
+                at_cp16(dst + F::PART, src + v_off, at >= 0);
+            }
+        }
+        at_commit();
+    };
+    locate(c0); locate(c0 + 1);
+    __syncthreads();
+    request(c0); request(c0 + 1);
+    for (int r = r0 + kh * (16 / KH); r < r0 + (kh + 1) * (16 / KH); ++r) {
+        const float unit = put_query<T, HD, LD>(a, s_row[r], sm, r, ROWS * HD);
+        if (lane == 0) s_unit[r] = unit;
+    }
+    __syncthreads();
+    const int32_t pos[2] = {s_row[r0 + g].pos, s_row[r0 + g + 8].pos};
+    const float scl[2] = {s_unit[r0 + g] * a.scale, s_unit[r0 + g + 8] * a.scale};
+    float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+    // the warp's own rows: positions that none of them sees are left out
+    int32_t w_lo = x.hi, w_hi = -1;
+    for (int r = r0; r < r0 + 16; ++r) if (s_row[r].pos >= 0) { w_lo = min(w_lo, s_row[r].pos); w_hi = max(w_hi, s_row[r].pos); }
+#pragma unroll 1
+    for (uint32_t c = c0; c < c1; ++c) {
+        at_wait<1>();
+        __syncthreads();
+        locate(c + 2);
+        const int p_in = kh * (CB / KH);
+        const int32_t p0 = chunk_at<CB>(x, c) + p_in, p1 = p0 + CB / KH - 1;
+        const bool some = p0 <= w_hi && (a.window == 0 || p1 > w_lo - (int32_t)a.window || (uint32_t)p0 < a.n_sink);
+        const bool all = p1 <= w_lo && (a.window == 0 || p0 > w_hi - (int32_t)a.window || (uint32_t)p1 < a.n_sink);
+        if (some) {
+            const uint32_t k_s = tiles_s + (c & 1) * 2 * F::PART;
+            const float* kf = reinterpret_cast<const float*>(tiles + (c & 1) * 2 * F::PART);
+            float s[NT][4], alpha[2];
+            if constexpr (H) scores_h<HD, NT>(s, q_s, ROWS * HD, r0, k_s, p_in);
+            else scores_f<HD, LD, NT>(s, reinterpret_cast<const float*>(sm), r0, kf, p_in);
+            weights<NT>(s, a, all, pos, scl, p0, m, l, alpha);
+            if constexpr (H) values_h<HD, NT>(o, s, alpha, k_s + F::PART, p_in);
+            else values_f<HD, LD, NT>(o, s, alpha, kf + CB * LD, p_in);
+        }
+        __syncthreads();
+        request(c + 2);
+    }
+    at_wait<0>();
+    finish<T, HD, ROWS, KH>(a, x, s_row, t, kvh, split, sharers, kh, r0, o, m, l, reinterpret_cast<float*>(sm), s_end);
+}
+
+template <typename K>
+static int launch_attn(K kernel, bool& set, const AttnArgs& a, uint32_t tiles, int threads, int smem) {
     if (!set) {
-        if (cudaFuncSetAttribute((const void*)k_attn_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM) != cudaSuccess)
+        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot raise the shared-memory limit");
         set = true;
     }
-    k_attn_few<T, HD><<<dim3(tiles * a.splits, a.geo.n_kv), F::W * 32, F::SMEM, g.stream>>>(a);
-    return ADAMAH_OK;
+    kernel<<<dim3(tiles * a.splits, a.geo.n_kv), threads, smem, g.stream>>>(a);
+    count_launch();
+    return check_launch("map_attn_kv");
+}
+template <typename T, int HD>
+static int launch_few(const AttnArgs& a, uint32_t tiles) {
+    static bool set = false;
+    return launch_attn(k_attn_few<T, HD>, set, a, tiles, Few<T, HD>::W * 32, Few<T, HD>::SMEM);
+}
+template <typename T, int HD, int RG, int KH>
+static int launch_many(const AttnArgs& a, uint32_t tiles) {
+    static bool set = false;
+    return launch_attn(k_attn_many<T, HD, RG, KH>, set, a, tiles, RG * KH * 32, Many<T, HD, RG, KH>::SMEM);
+}
+template <typename T, int HD>
+static int launch_rows(const AttnArgs& a, uint32_t rows, uint32_t tiles) {
+    if constexpr (HD <= 128 && sizeof(T) == 2) if (rows == 128) return launch_many<T, HD, 8, 1>(a, tiles);
+    return rows == 64 ? launch_many<T, HD, 4, 2>(a, tiles) : rows == 32 ? launch_many<T, HD, 2, 4>(a, tiles) : launch_few<T, HD>(a, tiles);
 }
 template <typename T>
-static int launch_hd(AttnArgs& a, uint32_t tiles) {
+static int launch_hd(const AttnArgs& a, uint32_t rows, uint32_t tiles) {
     switch (a.geo.hd) {
-    case 32: return launch_few<T, 32>(a, tiles);
-    case 64: return launch_few<T, 64>(a, tiles);
-    case 128: return launch_few<T, 128>(a, tiles);
-    default: return launch_few<T, 256>(a, tiles);
+    case 32: return launch_rows<T, 32>(a, rows, tiles);
+    case 64: return launch_rows<T, 64>(a, rows, tiles);
+    case 128: return launch_rows<T, 128>(a, rows, tiles);
+    default: return launch_rows<T, 256>(a, rows, tiles);
     }
 }
 
@@ -367,20 +541,26 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     a.geo = kv->geo; a.pool = kv->pool; a.layer = layer; a.n_head = n_head; a.group = n_head / kv->d.n_head_kv;
     a.window = window > 0x7FFFFFFFu ? 0u : window; a.n_sink = n_sink; a.scale = scale; a.cap = cap; a.err = g.dev_err;
     a.part = kv->part; a.tickets = kv->tickets;
-    // Tiles: every entry has its rows * group / 16 and at most 15 / 16 more.
-    const uint64_t flat = (uint64_t)n_rows * a.group, tiles64 = (flat + 15ull * std::min(n_seqs, n_rows)) / 16;
-    if (tiles64 * a.geo.n_kv >= (1u << 30)) return fail(ADAMAH_ERR_INVALID, "attn_kv: %u rows of %u heads", n_rows, n_head);
-    const uint32_t tiles = (uint32_t)tiles64, ctas = tiles * a.geo.n_kv;
-    // Splits: as many CTAs as the GPU holds twice over, no more than the workspace has room for.  How far the sequences reach
+    // Tiles: every entry has its rows * group / ROWS and a part of one more.
+    const uint32_t entries = std::min(n_seqs, n_rows), sms = (uint32_t)g.sm_count;
+    const uint64_t flat = (uint64_t)n_rows * a.group;
+    auto tiles_of = [&](uint64_t rows) { return (flat + (rows - 1) * entries) / rows; };
+    if (tiles_of(16) * a.geo.n_kv >= (1u << 30)) return fail(ADAMAH_ERR_INVALID, "attn_kv: %u rows of %u heads", n_rows, n_head);
+    // Rows of a tile: 16 where the entries have no more, else the widest whose tiles still give every SM one.  A wide tile reads
+    // the cache less often; below one tile per SM the time is that of the longest tile.
+    uint32_t rows = 16;
+    if (flat > 16ull * entries)
+        for (rows = kv->elem == 2 && a.geo.hd <= 128 ? 128 : 64; rows > 32; rows /= 2)
+            if (flat / rows * a.geo.n_kv >= sms) break;
+    const uint32_t tiles = (uint32_t)tiles_of(rows), ctas = tiles * a.geo.n_kv;
+    // Splits: as many CTAs as the GPU holds at once, no more than the workspace has room for.  How far the sequences reach
     // only decides the launch; a graph that is replayed later divides what there is then.
     uint32_t reach = kv->pages.longest();
     if (a.window) reach = (uint32_t)std::min<uint64_t>(reach, (uint64_t)a.window + n_sink);
-    a.least = 8;
-    a.splits = std::max(1u, std::min({(uint32_t)g.sm_count * 2 / ctas, KV_SPLIT_CTAS / ctas, (reach + 127) / 128}));
-    const int rc0 = kv->elem == 2 ? launch_hd<__half>(a, tiles) : launch_hd<float>(a, tiles);
-    if (rc0) return rc0;
-    count_launch();
-    const int rc = check_launch("map_attn_kv");
+    const uint32_t chunk = rows == 16 ? 16 : kv->elem == 2 ? 64 : 32;
+    a.least = 128 / chunk;
+    a.splits = std::max(1u, std::min({sms * (rows == 16 ? 2 : 1) / ctas, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / ctas, (reach + 127) / 128}));
+    const int rc = kv->elem == 2 ? launch_hd<__half>(a, rows, tiles) : launch_hd<float>(a, rows, tiles);
     end_of_op();
     return rc;
 }
