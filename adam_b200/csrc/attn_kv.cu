@@ -19,8 +19,6 @@
 
 namespace ab {
 
-constexpr float FLT_TOP = 3.402823466e+38f;
-
 // 16-byte words of 16-bit rows, so that eight neighbouring rows of one column lie in different banks
 template <int HD>
 __device__ __forceinline__ int swz(int r, int ch) { return HD >= 64 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3); }
@@ -194,106 +192,30 @@ __device__ __forceinline__ void values_f(float (&o)[HD / 8][4], const float (&s)
     }
 }
 
-// What is left at the end: PLANES sets of warps hold sums over different positions of the same ROWS rows (set k's warps the row
-// groups r0 = 0, 16, ..).  They meet in shared memory (`merge`), then the CTAs that share the tile in global memory, the last one
-// to arrive adds up in their order and writes the results; rows that are not finite are done once more, by themselves.
-template <int ROWS, int PLANES>
-struct End { float m[PLANES][ROWS], l[PLANES][ROWS]; uint32_t bad[(ROWS + 31) / 32], ticket; };
-
+// The warps' results into shared memory, then the rest of the way.
 template <typename T, int HD, int ROWS, int PLANES>
 __device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
                                        int plane, int r0, const float (&o)[HD / 8][4], const float (&m)[2], float (&l)[2], float* merge, End<ROWS, PLANES>& end) {
     constexpr int LM = HD + 4;
     constexpr float UNIT = sizeof(T) == 2 ? 1.f / 256.f : 1.f;
-    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         if (q4 == 0) { end.m[plane][r0 + g + 8 * h] = m[h]; end.l[plane][r0 + g + 8 * h] = l[h]; }
     }
-    if (tid < (ROWS + 31) / 32) end.bad[tid] = 0;
     __syncthreads();                                     // (and nobody reads what `merge` lies on any more)
-    float best[2], sum[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = r0 + g + 8 * h;
-        best[h] = -INFINITY; sum[h] = 0.f;
-#pragma unroll
-        for (int w = 0; w < PLANES; ++w) best[h] = max_nan(best[h], end.m[w][r]);
-        const float ref = best[h] == -INFINITY ? 0.f : best[h];
-#pragma unroll
-        for (int w = 0; w < PLANES; ++w) sum[h] += end.l[w][r] * expf(end.m[w][r] - ref);
-        const float f = expf(m[h] - ref) * UNIT;
+        const float f = end.template factor<false>(plane, r) * UNIT;
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j)
             *reinterpret_cast<float2*>(merge + (plane * ROWS + r) * LM + 8 * j + 2 * q4) = make_float2(o[j][2 * h] * f, o[j][2 * h + 1] * f);
     }
-    __syncthreads();
-    if (plane == 0 && q4 == 0)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) { end.m[0][r0 + g + 8 * h] = best[h]; end.l[0][r0 + g + 8 * h] = sum[h]; }
-    __syncthreads();
-    const uint32_t live = min((uint32_t)ROWS, x.n * a.group - x.first);
-    auto value = [&](uint32_t r, uint32_t d) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < PLANES; ++w) v += merge[(w * ROWS + r) * LM + d];
-        return v;
-    };
-    if (sharers > 1) {
-        const size_t tile = (size_t)t * a.geo.n_kv + kvh, step = (size_t)ROWS * (HD + 2);
-        float* mine = a.part + (tile * a.splits + split) * step;
-        for (uint32_t i = tid; i < live * HD; i += nt) mine[ROWS * 2 + i] = value(i / HD, i % HD);
-        if (tid < (int)live) { mine[2 * tid] = end.m[0][tid]; mine[2 * tid + 1] = end.l[0][tid]; }
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) end.ticket = atomicInc(a.tickets + tile, sharers - 1);
-        __syncthreads();
-        if (end.ticket != sharers - 1) return;
-        __threadfence();
-        const float* all = a.part + tile * a.splits * step;
-        for (uint32_t r = tid; r < live; r += nt) {
-            float b = -INFINITY, z = 0.f;
-            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, __ldcg(all + k * step + 2 * r));
-            const float ref = b == -INFINITY ? 0.f : b;
-            for (uint32_t k = 0; k < sharers; ++k) z += __ldcg(all + k * step + 2 * r + 1) * expf(__ldcg(all + k * step + 2 * r) - ref);
-            end.m[0][r] = ref; end.l[0][r] = z;
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < live * HD; i += nt) {
-            const uint32_t r = i / HD;
-            float v = 0.f;
-#pragma unroll 8
-            for (uint32_t k = 0; k < sharers; ++k) v = fmaf(__ldcg(all + k * step + ROWS * 2 + i), expf(__ldcg(all + k * step + 2 * r) - end.m[0][r]), v);
-            merge[r * LM + i % HD] = v;
-        }
-        __syncthreads();
-    }
-    for (uint32_t i = tid; i < live * HD; i += nt) {
-        const uint32_t r = i / HD, d = i % HD;
-        const float v = (sharers > 1 ? merge[r * LM + d] : value(r, d)) / end.l[0][r];
-        if (rows[r].pos < 0) continue;
-        if (!(fabsf(v) <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
-        merge[r * LM + d] = v;
-    }
-    __syncthreads();
-    auto bad = [&](uint32_t r) { return end.bad[r >> 5] >> (r & 31) & 1u; };
-    for (uint32_t i = tid; i < live * HD; i += nt) {
-        const uint32_t r = i / HD, d = i % HD;
-        if (rows[r].pos >= 0 && !bad(r)) a.act[rows[r].o + d] = merge[r * LM + d];
-    }
-    for (uint32_t r = tid >> 5; r < live; r += nt >> 5)
-        if (bad(r)) attend_row<T, HD>(a, x, rows[r], kvh);
+    settle<T, HD, ROWS, PLANES, false>(a, x, rows, t, kvh, split, sharers, merge, end);
 }
-// This CTA's chunks of the tile; false: it has none
-__device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, uint32_t split, uint32_t& sharers, uint32_t& c0, uint32_t& c1) {
-    const uint32_t each = max((x.chunks + a.splits - 1) / a.splits, a.least);
-    sharers = (x.chunks + each - 1) / each;
-    c0 = split * each; c1 = min(x.chunks, c0 + each);
-    return split < sharers;
-}
-
 // ---- few rows: 16 per tile -------------------------------------------------------------------------------------------
 // Every warp has chunks of 16 positions of its own (chunk w, w + W, ..), the next ones under way in STAGES slots of
 // shared memory, and its own running maxima, sums and outputs; nothing in the loop waits for another warp.  Bound by HBM: the tensor
@@ -505,7 +427,8 @@ static int launch_many(const AttnArgs& a, uint32_t tiles) {
 }
 template <typename T, int HD>
 static int launch_rows(const AttnArgs& a, uint32_t rows, uint32_t tiles) {
-    if constexpr (HD <= 128 && sizeof(T) == 2) if (rows == 128) return launch_many<T, HD, 8, 1>(a, tiles);
+    if constexpr (HD == 32 && sizeof(T) == 2) if (rows == 128) return launch_many<T, HD, 8, 1>(a, tiles);
+    if (rows == 128) return launch_attn_tc(a, tiles);
     return rows == 64 ? launch_many<T, HD, 4, 2>(a, tiles) : rows == 32 ? launch_many<T, HD, 2, 4>(a, tiles) : launch_few<T, HD>(a, tiles);
 }
 template <typename T>
@@ -539,7 +462,8 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     if (!n_rows || !n_seqs) return ADAMAH_OK;
     a.act = (float*)m->buf; a.n_act = m->n_elems; a.l_q = hlocs(q_h); a.l_out = hlocs(out_h);
     a.geo = kv->geo; a.pool = kv->pool; a.layer = layer; a.n_head = n_head; a.group = n_head / kv->d.n_head_kv;
-    a.window = window > 0x7FFFFFFFu ? 0u : window; a.n_sink = n_sink; a.scale = scale; a.cap = cap; a.err = g.dev_err;
+    a.window = window >= 1u << 30 ? 0u : window;         // no sequence is that long
+    a.n_sink = n_sink; a.scale = scale; a.cap = cap; a.err = g.dev_err;
     a.part = kv->part; a.tickets = kv->tickets;
     // Tiles: every entry has its rows * group / ROWS and a part of one more.
     const uint32_t entries = std::min(n_seqs, n_rows), sms = (uint32_t)g.sm_count;
@@ -557,7 +481,7 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     // only decides the launch; a graph that is replayed later divides what there is then.
     uint32_t reach = kv->pages.longest();
     if (a.window) reach = (uint32_t)std::min<uint64_t>(reach, (uint64_t)a.window + n_sink);
-    const uint32_t chunk = rows == 16 ? 16 : kv->elem == 2 ? 64 : 32;
+    const uint32_t chunk = rows == 16 ? 16 : rows == 128 && a.geo.hd > 32 ? 128 : kv->elem == 2 ? 64 : 32;
     a.least = 128 / chunk;
     a.splits = std::max(1u, std::min({sms * (rows == 16 ? 2 : 1) / ctas, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / ctas, (reach + 127) / 128}));
     const int rc = kv->elem == 2 ? launch_hd<__half>(a, rows, tiles) : launch_hd<float>(a, rows, tiles);

@@ -191,4 +191,108 @@ __device__ __noinline__ void attend_row(const AttnArgs& a, const AttnTile x, con
     for (int j = 0; j < N; ++j) a.act[row.o + lane * N + j] = o[j] / l;
 }
 
+constexpr float FLT_TOP = 3.402823466e+38f;
+
+// What is left at the end of a tile: PLANES sets of sums over different positions of the same ROWS rows, with the maxima that
+// they are relative to (BASE2: in units of ln 2).  They meet in shared memory (`merge`, rows of HD + 4 floats, each set's sums
+// times factor()), then the CTAs that share the tile in global memory: the last one to arrive adds up in their order and
+// writes the results.  Rows that are not finite are done once more, by themselves.
+template <int ROWS, int PLANES>
+struct End {
+    float m[PLANES][ROWS], l[PLANES][ROWS];
+    uint32_t bad[(ROWS + 31) / 32], ticket;
+    __device__ __forceinline__ float best(int r) const {
+        float b = m[0][r];
+#pragma unroll
+        for (int w = 1; w < PLANES; ++w) b = max_nan(b, m[w][r]);
+        return b;
+    }
+    template <bool BASE2> __device__ static __forceinline__ float weight(float from, float to) {   // of what is relative to `from`, relative to `to`
+        const float d = from - (to == -INFINITY ? 0.f : to);
+        return BASE2 ? exp2f(d) : expf(d);
+    }
+    template <bool BASE2> __device__ __forceinline__ float factor(int plane, int r) const { return weight<BASE2>(m[plane][r], best(r)); }
+};
+
+// By all threads of the CTA, m, l and merge written.
+template <typename T, int HD, int ROWS, int PLANES, bool BASE2>
+__device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
+                                       float* merge, End<ROWS, PLANES>& end) {
+    using E = End<ROWS, PLANES>;
+    constexpr int LM = HD + 4;
+    const int tid = threadIdx.x, nt = blockDim.x;
+    if (tid < (ROWS + 31) / 32) end.bad[tid] = 0;
+    __syncthreads();
+    for (int r = tid; r < ROWS; r += nt) {               // a row's maximum and sum into the first set's place
+        const float b = end.best(r);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < PLANES; ++w) sum += end.l[w][r] * E::template weight<BASE2>(end.m[w][r], b);
+        end.m[0][r] = b; end.l[0][r] = sum;
+    }
+    __syncthreads();
+    const uint32_t live = min((uint32_t)ROWS, x.n * a.group - x.first);
+    auto value = [&](uint32_t r, uint32_t d) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < PLANES; ++w) v += merge[(w * ROWS + r) * LM + d];
+        return v;
+    };
+    if (sharers > 1) {
+        const size_t tile = (size_t)t * a.geo.n_kv + kvh, step = (size_t)ROWS * (HD + 2);
+        float* mine = a.part + (tile * a.splits + split) * step;
+        for (uint32_t i = tid; i < live * HD; i += nt) mine[ROWS * 2 + i] = value(i / HD, i % HD);
+        for (uint32_t r = tid; r < live; r += nt) { mine[2 * r] = end.m[0][r]; mine[2 * r + 1] = end.l[0][r]; }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) end.ticket = atomicInc(a.tickets + tile, sharers - 1);
+        __syncthreads();
+        if (end.ticket != sharers - 1) return;
+        __threadfence();
+        const float* all = a.part + tile * a.splits * step;
+        for (uint32_t r = tid; r < live; r += nt) {
+            float b = -INFINITY, z = 0.f;
+            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, __ldcg(all + k * step + 2 * r));
+            for (uint32_t k = 0; k < sharers; ++k) z += __ldcg(all + k * step + 2 * r + 1) * E::template weight<BASE2>(__ldcg(all + k * step + 2 * r), b);
+            end.m[0][r] = b; end.l[0][r] = z;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < live * HD; i += nt) {
+            const uint32_t r = i / HD;
+            float v = 0.f;
+#pragma unroll 8
+            for (uint32_t k = 0; k < sharers; ++k)
+                v = fmaf(__ldcg(all + k * step + ROWS * 2 + i), E::template weight<BASE2>(__ldcg(all + k * step + 2 * r), end.m[0][r]), v);
+            merge[r * LM + i % HD] = v;
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = tid; i < live * HD; i += nt) {
+        const uint32_t r = i / HD, d = i % HD;
+        const float v = (sharers > 1 ? merge[r * LM + d] : value(r, d)) / end.l[0][r];
+        if (rows[r].pos < 0) continue;
+        if (!(fabsf(v) <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
+        merge[r * LM + d] = v;
+    }
+    __syncthreads();
+    auto bad = [&](uint32_t r) { return end.bad[r >> 5] >> (r & 31) & 1u; };
+    for (uint32_t i = tid; i < live * HD; i += nt) {
+        const uint32_t r = i / HD, d = i % HD;
+        if (rows[r].pos >= 0 && !bad(r)) a.act[rows[r].o + d] = merge[r * LM + d];
+    }
+    for (uint32_t r = tid >> 5; r < live; r += nt >> 5)
+        if (bad(r)) attend_row<T, HD>(a, x, rows[r], kvh);
+}
+// This CTA's chunks of the tile; false: it has none
+__device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, uint32_t split, uint32_t& sharers, uint32_t& c0, uint32_t& c1) {
+    const uint32_t each = max((x.chunks + a.splits - 1) / a.splits, a.least);
+    sharers = (x.chunks + each - 1) / each;
+    c0 = split * each; c1 = min(x.chunks, c0 + each);
+    return split < sharers;
+}
+
+
+// The tcgen05 form, 128 rows to a tile, over an fp16 cache with heads of 64 or 128 (attn_kv_tc.cu).
+int launch_attn_tc(const AttnArgs& a, uint32_t tiles);
+
 }  // namespace ab

@@ -1,0 +1,319 @@
+// Attention of many rows over a paged fp16 cache on the 5th-generation tensor cores (see attn_kv.cu for the operator and the
+// precision of its operands).
+//
+// A CTA has 128 rows (a token's query heads of one key head are neighbours) and walks the positions in chunks of 128:
+//   S = (Q_hi + Q_lo) K^T    tcgen05.mma, both operands in shared memory, into 128 columns of tensor memory
+//   P = 2^(k S - m + 8)      a row to a thread: S read twice (maximum, weights), P as two fp16 terms over S, column for column
+//   O' = (P_hi + P_lo) V     tcgen05.mma, P from tensor memory, V from shared memory as it lies there (its positions are the rows)
+//   O = O alpha + O'         in registers: a sum that stays in the tensor core for many chunks would lose bits (attn_kv.cu)
+// Two warpgroups take the even and the odd chunks, each with its own S / P, O' and running maximum, so that the tensor core
+// works on one's products while the other is at its weights; they merge at the end.  Three warps fetch keys and values
+// (16 bytes at a time, so that pages may end anywhere), one thread issues the products.  Bound by the tensor core, which has two
+// products where 16-bit operands would have one; the weights need about as many cycles of the other units.
+#include "attn_kv.cuh"
+#include "gemv_mma.cuh"
+
+namespace ab {
+
+constexpr int TC_ROWS = 128, TC_CB = 128, TC_THREADS = 384, TC_LOADERS = 96;
+constexpr uint32_t TC_BLOCK = 128 * 128;             // 128 rows (or positions) of 64 values: 128 bytes each, in the 128-byte swizzle
+
+template <int HD>
+struct AttnTc {
+    static constexpr uint32_t PLANE = HD / 64 * TC_BLOCK;                       // a tile of 128 rows
+    static constexpr uint32_t Q = 0, K = 2 * PLANE, V = K + 2 * PLANE, END = V + 2 * PLANE;      // two planes of Q, two stages of K and V
+    static constexpr uint32_t MERGE = 2 * TC_ROWS * (HD + 4) * 4;
+    static constexpr uint32_t SMEM = (END > MERGE ? END : MERGE) + 1024;        // + alignment
+};
+
+// Value d of row r in a tile
+__device__ __forceinline__ uint32_t tc_at(int r, int d) { return (uint32_t)(d >> 6) * TC_BLOCK + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2; }
+
+// Matrix descriptors with the 128-byte swizzle (2 at bit 61) and this architecture's version (1 at bit 46); addresses and
+// distances in 16-byte units.  Rows along M or N, values along K (Q, K): groups of 8 rows are 1024 bytes apart, the 16 values of an
+// instruction 32 bytes of a row.  The other way round (V as the second operand: N along a row, positions are K): groups of 8
+// positions 1024 bytes apart, blocks of 64 columns TC_BLOCK, the 16 positions of an instruction 2048 bytes.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16: D = f32 (1 at bit 4), A = B = f16, second operand with N along its rows (bit 16), N / 8 at bit 17, M / 16 at bit 24
+template <int N, bool N_ROWS> constexpr uint32_t ATC_IDESC = (1u << 4) | (N_ROWS ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+
+__device__ __forceinline__ void atc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void atc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void atc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void atc_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ bool atc_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void atc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void atc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void atc_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 32 consecutive columns of this thread's lane (valid after atc_ld_wait), 16 to them
+__device__ __forceinline__ void atc_ld32(uint32_t t, float (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
+                   "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]),
+                   "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+                 : "r"(t) : "memory");
+}
+__device__ __forceinline__ void atc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void atc_st16(uint32_t t, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void atc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float atc_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+// Columns of tensor memory: S / P of the even chunks, of the odd ones, then O' of each
+constexpr uint32_t COL_S = 0, COL_O = 256;
+
+template <int HD>
+__global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ AttnArgs a) {
+    using F = AttnTc<HD>;
+    extern __shared__ uint8_t raw[];
+    __shared__ AttnRow s_row[TC_ROWS];
+    __shared__ float s_unit[TC_ROWS];
+    __shared__ uint32_t s_scratch[TC_THREADS / 32 + 2], s_tmem, s_dead;
+    __shared__ int64_t s_where[2][TC_CB];
+    __shared__ End<TC_ROWS, 2> s_end;
+    // chunk c, stage c & 1: its keys are there / its scores are (and its keys read); its values / its weights / its output (and its values read)
+    __shared__ __align__(8) uint64_t b_k[2], b_s[2], b_v[2], b_p[2], b_o[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = gridDim.x / a.splits - 1 - blockIdx.x / a.splits;   // late rows see more: first
+    AttnTile x;
+    if (!find_tile<TC_ROWS, TC_CB>(a, t, kvh, x, s_row, s_scratch)) return;
+    uint32_t sharers, c0, c1;
+    if (!share_out(a, x, split, sharers, c0, c1)) return;
+    const int n = (int)(c1 - c0);
+    uint8_t* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const uint32_t sm_s = smem_u32(sm);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], TC_LOADERS); mbar_init(&b_s[i], 1); mbar_init(&b_v[i], TC_LOADERS); mbar_init(&b_p[i], 128); mbar_init(&b_o[i], 1); }
+        s_dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 11) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // queries: two fp16 terms of the row times a power of two (with the sign of the scale)
+    for (int r = warp; r < TC_ROWS; r += TC_THREADS / 32) {
+        const AttnRow row = s_row[r];
+        float v[HD / 32], most = 0.f, up, down;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) { v[j] = row.pos >= 0 ? a.act[row.q + lane + 32 * j] : 0.f; most = fmaxf(most, fabsf(v[j])); }
+        row_scale(warp_max(most), up, down);
+        if (lane == 0) s_unit[r] = down;
+        if (a.scale < 0.f) up = -up;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            const float y = v[j] * up;
+            const __half hi = __float2half_rn(y);
+            uint8_t* p = sm + F::Q + tc_at(r, lane + 32 * j);
+            *reinterpret_cast<__half*>(p) = hi;
+            *reinterpret_cast<__half*>(p + F::PLANE) = __float2half_rn(y - __half2float(hi));
+        }
+    }
+    atc_proxy_fence();
+    atc_fence_before();
+    __syncthreads();
+    atc_fence_after();
+    const uint32_t tmem = s_tmem;
+    bool dead = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {        // bounded: what comes later then does not wait any more
+        if (!dead && !mbar_wait(bar, parity)) { dead = true; s_dead = 1; atomicOr(a.err, DEVERR_WAIT); }
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp < 11) {
+            // ---- keys and values ----
+            const int me = tid - 256;
+            const __half* const pool = reinterpret_cast<const __half*>(a.pool);
+            const size_t v_off = (size_t)a.geo.n_kv * a.geo.page * HD;
+            constexpr int WPR = HD / 8;                      // 16-byte words of a row
+            uint64_t* owed = nullptr;                        // whose copies are under way and not yet announced
+            auto announce = [&]() { atc_proxy_fence(); atc_arrive(owed); owed = nullptr; };
+            auto fetch = [&](int c, uint32_t base, size_t off, uint64_t* free, uint64_t* full) {
+                if (c >= 2 && !atc_try(free, (uint32_t)((c >> 1) - 1) & 1u)) {
+                    if (owed) { at_wait<0>(); announce(); }
+                    wait(free, (uint32_t)((c >> 1) - 1) & 1u);
+                }
+#pragma unroll 4
+                for (int w = me; w < TC_CB * WPR; w += TC_LOADERS) {
+                    const int r = w / WPR, ch = w % WPR;
+                    const int64_t at = s_where[c & 1][r];
+                    at_cp16(sm_s + base + (uint32_t)(c & 1) * F::PLANE + tc_at(r, ch * 8), pool + (at < 0 ? 0 : (size_t)at + off) + ch * 8, at >= 0);
+                }
+                at_commit();
+                if (owed) { at_wait<1>(); announce(); }
+                owed = full;
+            };
+            for (int c = 0; c < n; ++c) {
+                const int32_t p0 = chunk_at<TC_CB>(x, c0 + c);
+                for (int r = me; r < TC_CB; r += TC_LOADERS) s_where[c & 1][r] = tile_position(a, x, kvh, p0 + r);
+                asm volatile("bar.sync 1, %0;" :: "n"(TC_LOADERS) : "memory");
+                fetch(c, F::K, 0, &b_s[c & 1], &b_k[c & 1]);
+                fetch(c, F::V, v_off, &b_o[c & 1], &b_v[c & 1]);
+            }
+            at_wait<0>();
+            if (owed) announce();
+        } else if (lane == 0) {
+            // ---- products: S of chunk c + 1 goes ahead of O' of chunk c ----
+            auto scores = [&](int c) {
+                const int b = c & 1;
+                wait(&b_k[b], (uint32_t)(c >> 1) & 1u);
+                atc_fence_after();
+                if (dead) return;
+#pragma unroll
+                for (int pass = 0; pass < 2; ++pass)         // the low terms first: they are added while the sum is small
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint32_t off = (uint32_t)(k >> 2) * TC_BLOCK + (k & 3) * 32;
+                        atc_mma_ss(tmem + COL_S + b * 128, tc_desc(sm_s + F::Q + (1 - pass) * F::PLANE + off, 16, 1024),
+                                   tc_desc(sm_s + F::K + b * F::PLANE + off, 16, 1024), ATC_IDESC<128, false>, pass + k > 0);
+                    }
+                atc_commit(&b_s[b]);
+            };
+            auto output = [&](int c) {
+                const int b = c & 1;
+                wait(&b_v[b], (uint32_t)(c >> 1) & 1u);
+                wait(&b_p[b], (uint32_t)(c >> 1) & 1u);
+                atc_fence_after();
+                if (dead) return;
+#pragma unroll
+                for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+                    for (int k = 0; k < TC_CB / 16; ++k)
+                        atc_mma_ts(tmem + COL_O + b * HD, tmem + COL_S + b * 128 + (k >> 1) * 32 + (1 - pass) * 16 + (k & 1) * 8,
+                                   tc_desc(sm_s + F::V + b * F::PLANE + k * 2048, TC_BLOCK, 1024), ATC_IDESC<HD, true>, pass + k > 0);
+                atc_commit(&b_o[b]);
+            };
+            scores(0);
+            for (int c = 0; c < n; ++c) {
+                if (c + 1 < n) scores(c + 1);
+                output(c);
+            }
+        }
+        __syncwarp();
+        __syncthreads();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        // ---- weights and sums: a row to a thread, every other chunk ----
+        const int w = warp >> 2, r = tid & 127;
+        const uint32_t col = tmem + ((uint32_t)(warp & 3) << 21), s_col = col + COL_S + w * 128, o_col = col + COL_O + w * HD;
+        const int32_t pos = s_row[r].pos;
+        const float unit = s_unit[r] * fabsf(a.scale), k2 = unit * 1.4426950408889634f;      // scores to powers of two
+        const float rcap = a.cap > 0.f ? __frcp_rn(a.cap) : 0.f, cap2 = a.cap * 1.4426950408889634f;
+        float o[HD], m = -INFINITY, l = 0.f, alpha = 0.f;
+#pragma unroll
+        for (int d = 0; d < HD; ++d) o[d] = 0.f;
+        auto collect = [&](int c) {                          // O' of chunk c, which is relative to m
+            wait(&b_o[w], (uint32_t)(c >> 1) & 1u);
+            atc_fence_after();
+#pragma unroll
+            for (int d0 = 0; d0 < HD; d0 += 32) {
+                float v[32];
+                atc_ld32(o_col + d0, v);
+                atc_ld_wait();
+#pragma unroll
+                for (int d = 0; d < 32; ++d) o[d0 + d] = fmaf(o[d0 + d], alpha, v[d]);
+            }
+        };
+        for (int c = w; c < n; c += 2) {
+            if (c >= 2) collect(c - 2);
+            const int32_t p0 = chunk_at<TC_CB>(x, c0 + c);
+            const bool all = tile_sees(a, x, p0, TC_CB);
+            // position p0 + j is seen for j <= j1 and (j > j0 or j < js)
+            const int32_t j1 = pos - p0, j0 = a.window ? j1 - (int32_t)a.window : -1, js = (int32_t)min(a.n_sink, 0x40000000u) - p0;
+            wait(&b_s[w], (uint32_t)(c >> 1) & 1u);
+            atc_fence_after();
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int d0 = 0; d0 < TC_CB; d0 += 32) {
+                float v[32];
+                atc_ld32(s_col + d0, v);
+                atc_ld_wait();
+                if (all) {
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) mx = fmaxf(mx, v[d]);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) mx = fmaxf(mx, d0 + d <= j1 && (d0 + d > j0 || d0 + d < js) ? v[d] : -INFINITY);
+                }
+            }
+            mx = a.cap > 0.f ? cap2 * at_tanh(mx * (unit * rcap)) : mx * k2;
+            const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn, shift = 8.f - ref;       // times 256: the low terms stay clear of the subnormals
+            alpha = atc_exp2(m - ref);
+            m = mn;
+            float sum = 0.f;
+#pragma unroll 1
+            for (int d0 = 0; d0 < TC_CB; d0 += 32) {
+                float v[32];
+                atc_ld32(s_col + d0, v);
+                atc_ld_wait();
+                if (a.cap > 0.f) {
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) v[d] = atc_exp2(fmaf(at_tanh(v[d] * (unit * rcap)), cap2, shift));
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) v[d] = atc_exp2(fmaf(v[d], k2, shift));
+                }
+                if (!all)
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) if (!(d0 + d <= j1 && (d0 + d > j0 || d0 + d < js))) v[d] = 0.f;
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int d = 0; d < 16; ++d) { sum += v[2 * d] + v[2 * d + 1]; at_split_h(v[2 * d], v[2 * d + 1], hi[d], lo[d]); }
+                atc_st16(s_col + d0, hi);
+                atc_st16(s_col + d0 + 16, lo);
+            }
+            l = fmaf(l, alpha, sum);
+            atc_st_wait();
+            atc_fence_before();
+            atc_arrive(&b_p[w]);
+        }
+        if (n > w) collect((n - 1 - w) / 2 * 2 + w);
+        s_end.m[w][r] = m; s_end.l[w][r] = l * (1.f / 256.f);
+        atc_fence_before();
+        __syncthreads();                                     // all products are done, shared memory is free
+        const float f = s_end.factor<true>(w, r) * (1.f / 256.f);
+        float* to = reinterpret_cast<float*>(sm) + (w * TC_ROWS + r) * (HD + 4);
+#pragma unroll
+        for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
+    }
+    atc_fence_after();
+    __syncthreads();
+    if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+    if (s_dead) return;
+    settle<__half, HD, TC_ROWS, 2, true>(a, x, s_row, t, kvh, split, sharers, reinterpret_cast<float*>(sm), s_end);
+}
+
+template <int HD>
+static int launch_tc(const AttnArgs& a, uint32_t tiles) {
+    static bool set = false;
+    if (!set) {
+        if (cudaFuncSetAttribute((const void*)k_attn_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttnTc<HD>::SMEM) != cudaSuccess)
+            return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot raise the shared-memory limit");
+        set = true;
+    }
+    k_attn_tc<HD><<<dim3(tiles * a.splits, a.geo.n_kv), TC_THREADS, AttnTc<HD>::SMEM, g.stream>>>(a);
+    count_launch();
+    return check_launch("map_attn_kv");
+}
+int launch_attn_tc(const AttnArgs& a, uint32_t tiles) { return a.geo.hd == 64 ? launch_tc<64>(a, tiles) : launch_tc<128>(a, tiles); }
+
+}  // namespace ab

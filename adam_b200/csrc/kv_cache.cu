@@ -117,7 +117,7 @@ static int create(const adam_b200_kv_desc& desc, uint32_t id) {
     if (d.kv_dtype > 1) return fail(ADAMAH_ERR_INVALID, "kv_create: kv_dtype %u (0 = float32, 1 = float16)", d.kv_dtype);
     if (!d.n_layer || !d.n_head_kv || !d.n_pages || !d.max_seqs || !d.max_pages) return fail(ADAMAH_ERR_INVALID, "kv_create: empty shape");
     if (d.page_size > 1024 || d.n_head_kv > 1024 || d.n_layer > 4096 || d.n_pages > (1u << 28) || d.max_seqs > (1u << 20) ||
-        (uint64_t)d.max_pages * d.page_size >= (1ull << 31) || (uint64_t)d.max_seqs * d.max_pages >= (1ull << 31))
+        (uint64_t)d.max_pages * d.page_size >= (1ull << 30) || (uint64_t)d.max_seqs * d.max_pages >= (1ull << 31))
         return fail(ADAMAH_ERR_INVALID, "kv_create: shape out of range");
     const uint64_t plane = (uint64_t)d.page_size * d.head_dim, page_elems = plane * d.n_layer * 2 * d.n_head_kv;
     if (page_elems >= (1ull << 31)) return fail(ADAMAH_ERR_INVALID, "kv_create: a page of %llu elements", (unsigned long long)page_elems);
