@@ -16,6 +16,7 @@
 #include "attn_kv.cuh"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace ab {
 
@@ -193,7 +194,7 @@ __device__ __forceinline__ void values_f(float (&o)[HD / 8][4], const float (&s)
 }
 
 // The warps' results into shared memory, then the rest of the way.
-template <typename T, int HD, int ROWS, int PLANES>
+template <typename T, int HD, int ROWS, int PLANES, int THREADS, bool CLUSTER>
 __device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
                                        int plane, int r0, const float (&o)[HD / 8][4], const float (&m)[2], float (&l)[2], float* merge, End<ROWS, PLANES>& end) {
     constexpr int LM = HD + 4;
@@ -214,12 +215,13 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, con
         for (int j = 0; j < HD / 8; ++j)
             *reinterpret_cast<float2*>(merge + (plane * ROWS + r) * LM + 8 * j + 2 * q4) = make_float2(o[j][2 * h] * f, o[j][2 * h + 1] * f);
     }
-    settle<T, HD, ROWS, PLANES, false>(a, x, rows, t, kvh, split, sharers, merge, end);
+    settle<T, HD, ROWS, PLANES, THREADS, false, CLUSTER>(a, x, rows, t, kvh, split, sharers, merge, end);
 }
 // ---- few rows: 16 per tile -------------------------------------------------------------------------------------------
 // Every warp has chunks of 16 positions of its own (chunk w, w + W, ..), the next ones under way in STAGES slots of
 // shared memory, and its own running maxima, sums and outputs; nothing in the loop waits for another warp.  Bound by HBM: the tensor
 // cores are busy for a few percent.
+constexpr uint32_t FEW_CLUSTER = 16;                 // CTAs that share a tile as a cluster, at most
 template <typename T, int HD>
 struct Few {
     static constexpr int ROWS = 16, CB = 16, ROW_BYTES = HD * (int)sizeof(T);
@@ -232,7 +234,8 @@ struct Few {
     static_assert(SMEM <= 225 * 1024, "shared memory");
 };
 
-template <typename T, int HD>
+// CLUSTER: a tile's CTAs are a cluster
+template <typename T, int HD, bool CLUSTER>
 __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_constant__ AttnArgs a) {
     using F = Few<T, HD>;
     constexpr int ROWS = F::ROWS, CB = F::CB, W = F::W, LD = F::LD, STAGES = F::STAGES;
@@ -240,14 +243,15 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ AttnRow s_row[ROWS];
     __shared__ float s_unit[ROWS];
-    __shared__ uint32_t s_scratch[W + 2];
+    __shared__ Found s_found;
     __shared__ End<ROWS, W> s_end;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
     const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = blockIdx.x / a.splits;
     AttnTile x;
-    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_scratch)) return;
+    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_found)) return;
     uint32_t sharers, c0, c1;
-    if (!share_out(a, x, split, sharers, c0, c1)) return;
+    if (!share_out(a, x, split, sharers, c0, c1) && !CLUSTER) return;         // in a cluster it still takes its rows
+    c0 = min(c0, c1);
 
     uint8_t* const ring = sm + F::Q_BYTES + warp * STAGES * F::SLOT;
     const uint32_t ring_s = at_smem(ring), q_s = at_smem(sm);
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
         slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     at_wait<0>();
-    finish<T, HD, ROWS, W>(a, x, s_row, t, kvh, split, sharers, warp, 0, o, m, l, reinterpret_cast<float*>(sm + F::Q_BYTES), s_end);
+    finish<T, HD, ROWS, W, W * 32, CLUSTER>(a, x, s_row, t, kvh, split, sharers, warp, 0, o, m, l, reinterpret_cast<float*>(sm + F::Q_BYTES), s_end);
 }
 
 // ---- many rows: 32 to 128 per tile -----------------------------------------------------------------------------------
@@ -330,13 +334,13 @@ __global__ void __launch_bounds__(RG * KH * 32) k_attn_many(const __grid_constan
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ AttnRow s_row[ROWS];
     __shared__ float s_unit[ROWS];
-    __shared__ uint32_t s_scratch[RG * KH + 2];
+    __shared__ Found s_found;
     __shared__ int64_t s_where[2][CB];
     __shared__ End<ROWS, KH> s_end;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rg = warp % RG, kh = warp / RG, r0 = rg * 16, g = lane >> 2;
     const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = blockIdx.x / a.splits;
     AttnTile x;
-    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_scratch)) return;
+    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_found)) return;
     uint32_t sharers, c0, c1;
     if (!share_out(a, x, split, sharers, c0, c1)) return;
     uint8_t* const tiles = sm + F::Q_BYTES;              // chunk c: keys at (c & 1) * 2 PART, values behind them
@@ -401,29 +405,34 @@ __global__ void __launch_bounds__(RG * KH * 32) k_attn_many(const __grid_constan
         request(c + 2);
     }
     at_wait<0>();
-    finish<T, HD, ROWS, KH>(a, x, s_row, t, kvh, split, sharers, kh, r0, o, m, l, reinterpret_cast<float*>(sm), s_end);
+    finish<T, HD, ROWS, KH, THREADS, false>(a, x, s_row, t, kvh, split, sharers, kh, r0, o, m, l, reinterpret_cast<float*>(sm), s_end);
 }
 
 template <typename K>
-static int launch_attn(K kernel, bool& set, const AttnArgs& a, uint32_t tiles, int threads, int smem) {
+static int launch_attn(K kernel, bool& set, const AttnArgs& a, uint32_t tiles, int threads, int smem, bool cluster) {
     if (!set) {
-        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot raise the shared-memory limit");
+        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            (cluster && cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
+            return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot set the kernel's limits");
         set = true;
     }
-    kernel<<<dim3(tiles * a.splits, a.geo.n_kv), threads, smem, g.stream>>>(a);
+    const dim3 grid(tiles * a.splits, a.geo.n_kv);
+    if (cluster) launch_k_cluster(kernel, grid, dim3(threads), smem, g.stream, false, a.splits, false, a);
+    else kernel<<<grid, threads, smem, g.stream>>>(a);
     count_launch();
     return check_launch("map_attn_kv");
 }
 template <typename T, int HD>
 static int launch_few(const AttnArgs& a, uint32_t tiles) {
-    static bool set = false;
-    return launch_attn(k_attn_few<T, HD>, set, a, tiles, Few<T, HD>::W * 32, Few<T, HD>::SMEM);
+    static bool set[2] = {false, false};
+    using F = Few<T, HD>;
+    if (a.splits > 1 && a.splits <= FEW_CLUSTER) return launch_attn(k_attn_few<T, HD, true>, set[1], a, tiles, F::W * 32, F::SMEM, true);
+    return launch_attn(k_attn_few<T, HD, false>, set[0], a, tiles, F::W * 32, F::SMEM, false);
 }
 template <typename T, int HD, int RG, int KH>
 static int launch_many(const AttnArgs& a, uint32_t tiles) {
     static bool set = false;
-    return launch_attn(k_attn_many<T, HD, RG, KH>, set, a, tiles, RG * KH * 32, Many<T, HD, RG, KH>::SMEM);
+    return launch_attn(k_attn_many<T, HD, RG, KH>, set, a, tiles, RG * KH * 32, Many<T, HD, RG, KH>::SMEM, false);
 }
 template <typename T, int HD>
 static int launch_rows(const AttnArgs& a, uint32_t rows, uint32_t tiles) {
@@ -476,6 +485,7 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     if (flat > 16ull * entries)
         for (rows = kv->elem == 2 && a.geo.hd <= 128 ? 128 : 64; rows > 32; rows /= 2)
             if (flat / rows * a.geo.n_kv >= sms) break;
+    if (getenv("AT_ROWS")) rows = atoi(getenv("AT_ROWS"));
     const uint32_t tiles = (uint32_t)tiles_of(rows), ctas = tiles * a.geo.n_kv;
     // Splits: as many CTAs as the GPU holds at once, no more than the workspace has room for.  How far the sequences reach
     // only decides the launch; a graph that is replayed later divides what there is then.
@@ -484,6 +494,11 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     const uint32_t chunk = rows == 16 ? 16 : rows == 128 && a.geo.hd > 32 ? 128 : kv->elem == 2 ? 64 : 32;
     a.least = 128 / chunk;
     a.splits = std::max(1u, std::min({sms * (rows == 16 ? 2 : 1) / ctas, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / ctas, (reach + 127) / 128}));
+    if (rows == 16 && a.splits > 1) {                    // a cluster where that is enough: 2, 4, 8 or 16 of them
+        uint32_t c = 1;
+        while (c < a.splits && c < FEW_CLUSTER) c *= 2;
+        if (a.splits <= FEW_CLUSTER || (getenv("AT_CL"))) a.splits = c;
+    }
     const int rc = kv->elem == 2 ? launch_hd<__half>(a, rows, tiles) : launch_hd<float>(a, rows, tiles);
     end_of_op();
     return rc;

@@ -26,49 +26,47 @@ struct AttnTile {
     int32_t from;                                       // positions below it are seen by none but as first ones
 };
 
-// Tile t of the batch, by the whole CTA (`scratch`: a word per warp and two more); false: there is none, or nothing to do.
-// Fills rows[0 .. ROWS).  CHUNK: positions per chunk.
+// Tile t of the batch, by the whole CTA; false: there is none, or nothing to do.  Fills rows[0 .. ROWS).  CHUNK: positions per
+// chunk.  A chain of three dependent loads (entry, length, row offsets), each of 0.6 us and more, is what a short call waits
+// for: an entry's sequence and length are loaded with its rows, before the tile's entry is known.
+struct Found { uint32_t seq, row, n, first, len, warp[32]; };
 template <int ROWS, int CHUNK>
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t t, uint32_t kvh, AttnTile& x, AttnRow* rows, uint32_t* scratch) {
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t t, uint32_t kvh, AttnTile& x, AttnRow* rows, Found& f) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    uint32_t* const hit = scratch + warps;              // entry and tile of the entry; no tile: entry 0xFFFFFFFF
     uint32_t before = 0;
-    if (tid == 0) hit[0] = KV_NO_SEQ;
+    if (tid == 0) f.seq = KV_NO_SEQ;
     for (uint32_t e0 = 0; e0 < a.b.n_seqs; e0 += blockDim.x) {
         const uint32_t e = e0 + tid;
-        uint32_t n = 0;
-        if (e < a.b.n_seqs) {
-            const uint32_t s0 = a.b.start[e], s1 = a.b.start[e + 1];
-            n = s0 < s1 && s1 <= a.b.n_rows ? s1 - s0 : 0u;
-            if (s1 < s0 || s1 > a.b.n_rows) atomicOr(a.err, DEVERR_OOB_MAP);
-        }
-        const uint32_t tiles = (n * a.group + ROWS - 1) / ROWS;
+        uint32_t s0 = 0, s1 = 0, seq = KV_NO_SEQ, len = 0;
+        if (e < a.b.n_seqs) { s0 = a.b.start[e]; s1 = a.b.start[e + 1]; seq = a.b.seq[e]; }
+        if (seq < a.b.max_seqs) len = (uint32_t)a.b.lens[seq];
+        const bool fine = s0 <= s1 && s1 <= a.b.n_rows;
+        if (!fine) atomicOr(a.err, DEVERR_OOB_MAP);
+        const uint32_t n = fine ? s1 - s0 : 0u, tiles = (n * a.group + ROWS - 1) / ROWS;
         uint32_t incl = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += v; }
         __syncthreads();
-        if (lane == 31) scratch[warp] = incl;
+        if (lane == 31) f.warp[warp] = incl;
         __syncthreads();
         uint32_t at = before + incl - tiles;
-        for (uint32_t w = 0; w < warps; ++w) { if (w < warp) at += scratch[w]; before += scratch[w]; }
-        if (at <= t && t < at + tiles) { hit[0] = e; hit[1] = t - at; }
+        for (uint32_t w = 0; w < warps; ++w) { if (w < warp) at += f.warp[w]; before += f.warp[w]; }
+        if (at <= t && t < at + tiles) { f.seq = seq; f.row = s0; f.n = n; f.first = (t - at) * ROWS; f.len = len; }
         if (before > t) break;
     }
     __syncthreads();
-    const uint32_t e = hit[0];
-    if (e == KV_NO_SEQ) return false;
-    x.seq = a.b.seq[e];
+    x.seq = f.seq;
     if (x.seq == KV_NO_SEQ) return false;
     if (x.seq >= a.b.max_seqs) { if (tid == 0) atomicOr(a.err, DEVERR_OOB_MAP); return false; }
-    x.row = a.b.start[e]; x.n = a.b.start[e + 1] - x.row; x.first = hit[1] * ROWS;
+    x.row = f.row; x.n = f.n; x.first = f.first;
     x.pages = a.b.table + (size_t)x.seq * a.geo.max_pages;
-    const int32_t pos0 = a.b.lens[x.seq] - (int32_t)x.n;
+    const int32_t pos0 = (int32_t)f.len - (int32_t)x.n;
     const uint32_t last = min(x.first + ROWS, x.n * a.group) - 1;
     x.lo = max(pos0 + (int32_t)(x.first / a.group), 0); x.hi = pos0 + (int32_t)(last / a.group);
     for (uint32_t r = tid; r < ROWS; r += blockDim.x) {
         AttnRow y{0, 0, -1};
-        const uint32_t f = x.first + r, tok = f / a.group, head = kvh * a.group + f % a.group;
-        if (f <= last) {
+        const uint32_t k = x.first + r, tok = k / a.group, head = kvh * a.group + k % a.group;
+        if (k <= last) {
             const uint64_t oq = a.l_q[x.row + tok], oo = a.l_out[x.row + tok], len = (uint64_t)a.n_head * a.geo.hd;
             y.pos = pos0 + (int32_t)tok;
             if (y.pos < 0 || oq + len > a.n_act || oo + len > a.n_act) { y.pos = -1; atomicOr(a.err, DEVERR_OOB_MAP); }
@@ -195,8 +193,9 @@ constexpr float FLT_TOP = 3.402823466e+38f;
 
 // What is left at the end of a tile: PLANES sets of sums over different positions of the same ROWS rows, with the maxima that
 // they are relative to (BASE2: in units of ln 2).  They meet in shared memory (`merge`, rows of HD + 4 floats, each set's sums
-// times factor()), then the CTAs that share the tile in global memory: the last one to arrive adds up in their order and
-// writes the results.  Rows that are not finite are done once more, by themselves.
+// times factor()), then the CTAs that share the tile: through their shared memory where they are a cluster, each taking some of
+// the rows, else in global memory, where the last one to arrive adds up in their order.  Rows that are not finite are done once
+// more, by themselves.
 template <int ROWS, int PLANES>
 struct End {
     float m[PLANES][ROWS], l[PLANES][ROWS];
@@ -213,17 +212,23 @@ struct End {
     }
     template <bool BASE2> __device__ __forceinline__ float factor(int plane, int r) const { return weight<BASE2>(m[plane][r], best(r)); }
 };
+__device__ __forceinline__ const float* of_rank(const float* p, uint32_t rank) {     // the same place in another CTA's shared memory
+    uint64_t q;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(p), "r"(rank));
+    return reinterpret_cast<const float*>(q);
+}
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// By all threads of the CTA, m, l and merge written.
-template <typename T, int HD, int ROWS, int PLANES, bool BASE2>
+// By all THREADS of the CTA, m, l and merge written.  CLUSTER: the tile's CTAs (a.splits of them) are one.
+template <typename T, int HD, int ROWS, int PLANES, int THREADS, bool BASE2, bool CLUSTER>
 __device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
                                        float* merge, End<ROWS, PLANES>& end) {
     using E = End<ROWS, PLANES>;
-    constexpr int LM = HD + 4;
-    const int tid = threadIdx.x, nt = blockDim.x;
+    constexpr int LM = HD + 4, VPR = HD / 4, PER = (ROWS * VPR + THREADS - 1) / THREADS;       // values in fours; of a row, of a thread
+    const uint32_t tid = threadIdx.x;
     if (tid < (ROWS + 31) / 32) end.bad[tid] = 0;
     __syncthreads();
-    for (int r = tid; r < ROWS; r += nt) {               // a row's maximum and sum into the first set's place
+    for (int r = tid; r < ROWS; r += THREADS) {          // a row's maximum and sum into the first set's place
         const float b = end.best(r);
         float sum = 0.f;
 #pragma unroll
@@ -233,55 +238,74 @@ __device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, con
     __syncthreads();
     const uint32_t live = min((uint32_t)ROWS, x.n * a.group - x.first);
     auto value = [&](uint32_t r, uint32_t d) {
-        float v = 0.f;
+        float4 v = *reinterpret_cast<const float4*>(merge + r * LM + d);
 #pragma unroll
-        for (int w = 0; w < PLANES; ++w) v += merge[(w * ROWS + r) * LM + d];
+        for (int w = 1; w < PLANES; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(merge + (w * ROWS + r) * LM + d);
+            v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+        }
         return v;
     };
-    if (sharers > 1) {
-        const size_t tile = (size_t)t * a.geo.n_kv + kvh, step = (size_t)ROWS * (HD + 2);
+    auto add = [](float4& v, float f, float4 y) { v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y); v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w); };
+    uint32_t first = 0, every = 1;                       // this CTA's rows
+    if (CLUSTER && a.splits > 1) {
+        for (uint32_t i = tid; i < live * VPR; i += THREADS) *reinterpret_cast<float4*>(merge + i / VPR * LM + i % VPR * 4) = value(i / VPR, i % VPR * 4);
+        cluster_meet();
+        first = split; every = a.splits;
+    } else if (sharers > 1) {
+        const size_t tile = (size_t)t * a.geo.n_kv + kvh, step = (size_t)ROWS * (HD + 4);      // per row: the values, the maximum, the sum
         float* mine = a.part + (tile * a.splits + split) * step;
-        for (uint32_t i = tid; i < live * HD; i += nt) mine[ROWS * 2 + i] = value(i / HD, i % HD);
-        for (uint32_t r = tid; r < live; r += nt) { mine[2 * r] = end.m[0][r]; mine[2 * r + 1] = end.l[0][r]; }
+        for (uint32_t i = tid; i < live * VPR; i += THREADS) *reinterpret_cast<float4*>(mine + i / VPR * LM + i % VPR * 4) = value(i / VPR, i % VPR * 4);
+        for (uint32_t r = tid; r < live; r += THREADS) *reinterpret_cast<float2*>(mine + r * LM + HD) = make_float2(end.m[0][r], end.l[0][r]);
         __threadfence();
         __syncthreads();
         if (tid == 0) end.ticket = atomicInc(a.tickets + tile, sharers - 1);
         __syncthreads();
         if (end.ticket != sharers - 1) return;
         __threadfence();
-        const float* all = a.part + tile * a.splits * step;
-        for (uint32_t r = tid; r < live; r += nt) {
-            float b = -INFINITY, z = 0.f;
-            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, __ldcg(all + k * step + 2 * r));
-            for (uint32_t k = 0; k < sharers; ++k) z += __ldcg(all + k * step + 2 * r + 1) * E::template weight<BASE2>(__ldcg(all + k * step + 2 * r), b);
-            end.m[0][r] = b; end.l[0][r] = z;
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < live * HD; i += nt) {
-            const uint32_t r = i / HD;
-            float v = 0.f;
-#pragma unroll 8
-            for (uint32_t k = 0; k < sharers; ++k)
-                v = fmaf(__ldcg(all + k * step + ROWS * 2 + i), E::template weight<BASE2>(__ldcg(all + k * step + 2 * r), end.m[0][r]), v);
-            merge[r * LM + i % HD] = v;
-        }
-        __syncthreads();
     }
-    for (uint32_t i = tid; i < live * HD; i += nt) {
-        const uint32_t r = i / HD, d = i % HD;
-        const float v = (sharers > 1 ? merge[r * LM + d] : value(r, d)) / end.l[0][r];
-        if (rows[r].pos < 0) continue;
-        if (!(fabsf(v) <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
-        merge[r * LM + d] = v;
+    const float* all = a.part + ((size_t)t * a.geo.n_kv + kvh) * a.splits * ROWS * LM;
+    float4 out[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint32_t i = tid + j * THREADS, r = first + i / VPR * every, d = i % VPR * 4;
+        if (r >= live) break;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float z = 0.f;
+        if ((CLUSTER && a.splits > 1) || sharers > 1) {
+            float b = -INFINITY;
+            auto ml = [&](uint32_t k) {
+                if (CLUSTER) return make_float2(*of_rank(&end.m[0][r], k), *of_rank(&end.l[0][r], k));
+                return __ldcg(reinterpret_cast<const float2*>(all + ((size_t)k * ROWS + r) * LM + HD));
+            };
+#pragma unroll 4
+            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, ml(k).x);
+#pragma unroll 4
+            for (uint32_t k = 0; k < sharers; ++k) {
+                const float2 q = ml(k);
+                const float w = E::template weight<BASE2>(q.x, b);
+                z = fmaf(q.y, w, z);
+                add(v, w, CLUSTER ? *reinterpret_cast<const float4*>(of_rank(merge + r * LM + d, k)) : __ldcg(reinterpret_cast<const float4*>(all + ((size_t)k * ROWS + r) * LM + d)));
+            }
+        } else { v = value(r, d); z = end.l[0][r]; }
+        out[j] = make_float4(v.x / z, v.y / z, v.z / z, v.w / z);
+        const float most = max_nan(max_nan(fabsf(out[j].x), fabsf(out[j].y)), max_nan(fabsf(out[j].z), fabsf(out[j].w)));
+        if (rows[r].pos >= 0 && !(most <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
     }
     __syncthreads();
     auto bad = [&](uint32_t r) { return end.bad[r >> 5] >> (r & 31) & 1u; };
-    for (uint32_t i = tid; i < live * HD; i += nt) {
-        const uint32_t r = i / HD, d = i % HD;
-        if (rows[r].pos >= 0 && !bad(r)) a.act[rows[r].o + d] = merge[r * LM + d];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint32_t i = tid + j * THREADS, r = first + i / VPR * every, d = i % VPR * 4;
+        if (r >= live) break;
+        if (rows[r].pos < 0 || bad(r)) continue;
+        float* to = a.act + rows[r].o + d;
+        if (rows[r].o % 4 == 0) *reinterpret_cast<float4*>(to) = out[j];
+        else { to[0] = out[j].x; to[1] = out[j].y; to[2] = out[j].z; to[3] = out[j].w; }
     }
-    for (uint32_t r = tid >> 5; r < live; r += nt >> 5)
+    for (uint32_t r = first + (tid >> 5) * every; r < live; r += (THREADS >> 5) * every)
         if (bad(r)) attend_row<T, HD>(a, x, rows[r], kvh);
+    if (CLUSTER && a.splits > 1) cluster_meet();         // nobody leaves while its shared memory is read
 }
 // This CTA's chunks of the tile; false: it has none
 __device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, uint32_t split, uint32_t& sharers, uint32_t& c0, uint32_t& c1) {

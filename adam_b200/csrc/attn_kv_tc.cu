@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     extern __shared__ uint8_t raw[];
     __shared__ AttnRow s_row[TC_ROWS];
     __shared__ float s_unit[TC_ROWS];
-    __shared__ uint32_t s_scratch[TC_THREADS / 32 + 2], s_tmem, s_dead;
+    __shared__ uint32_t s_tmem, s_dead;
+    __shared__ Found s_found;
     __shared__ int64_t s_where[2][TC_CB];
     __shared__ End<TC_ROWS, 2> s_end;
     // chunk c, stage c & 1: its keys are there / its scores are (and its keys read); its values / its weights / its output (and its values read)
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = gridDim.x / a.splits - 1 - blockIdx.x / a.splits;   // late rows see more: first
     AttnTile x;
-    if (!find_tile<TC_ROWS, TC_CB>(a, t, kvh, x, s_row, s_scratch)) return;
+    if (!find_tile<TC_ROWS, TC_CB>(a, t, kvh, x, s_row, s_found)) return;
     uint32_t sharers, c0, c1;
     if (!share_out(a, x, split, sharers, c0, c1)) return;
     const int n = (int)(c1 - c0);
@@ -109,22 +110,37 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // queries: two fp16 terms of the row times a power of two (with the sign of the scale)
-    for (int r = warp; r < TC_ROWS; r += TC_THREADS / 32) {
-        const AttnRow row = s_row[r];
-        float v[HD / 32], most = 0.f, up, down;
+    // queries: two fp16 terms of the row times a power of two (with the sign of the scale), four rows of a warp under way at once
+    constexpr int W = TC_THREADS / 32, VPL = HD / 32, R4 = 4;
+#pragma unroll 1
+    for (int r1 = warp; r1 < TC_ROWS; r1 += R4 * W) {
+        float v[R4][VPL];
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) { v[j] = row.pos >= 0 ? a.act[row.q + lane + 32 * j] : 0.f; most = fmaxf(most, fabsf(v[j])); }
-        row_scale(warp_max(most), up, down);
-        if (lane == 0) s_unit[r] = down;
-        if (a.scale < 0.f) up = -up;
+        for (int j = 0; j < R4; ++j) {
+            const int r = r1 + j * W;
+            const bool on = r < TC_ROWS && s_row[r].pos >= 0;
+            const float* src = a.act + (on ? s_row[r].q : 0);
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-            const float y = v[j] * up;
-            const __half hi = __float2half_rn(y);
-            uint8_t* p = sm + F::Q + tc_at(r, lane + 32 * j);
-            *reinterpret_cast<__half*>(p) = hi;
-            *reinterpret_cast<__half*>(p + F::PLANE) = __float2half_rn(y - __half2float(hi));
+            for (int i = 0; i < VPL; ++i) v[j][i] = on ? src[lane + 32 * i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < R4; ++j) {
+            const int r = r1 + j * W;
+            if (r >= TC_ROWS) break;
+            float most = 0.f, up, down;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) most = fmaxf(most, fabsf(v[j][i]));
+            row_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))), up, down);
+            if (lane == 0) s_unit[r] = down;
+            if (a.scale < 0.f) up = -up;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const float y = v[j][i] * up;
+                const __half hi = __float2half_rn(y);
+                uint8_t* p = sm + F::Q + tc_at(r, lane + 32 * i);
+                *reinterpret_cast<__half*>(p) = hi;
+                *reinterpret_cast<__half*>(p + F::PLANE) = __float2half_rn(y - __half2float(hi));
+            }
         }
     }
     atc_proxy_fence();
@@ -299,7 +315,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     __syncthreads();
     if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     if (s_dead) return;
-    settle<__half, HD, TC_ROWS, 2, true>(a, x, s_row, t, kvh, split, sharers, reinterpret_cast<float*>(sm), s_end);
+    settle<__half, HD, TC_ROWS, 2, TC_THREADS, true, false>(a, x, s_row, t, kvh, split, sharers, reinterpret_cast<float*>(sm), s_end);
 }
 
 template <int HD>

@@ -127,7 +127,7 @@ static int create(const adam_b200_kv_desc& desc, uint32_t id) {
     kv->geo = KvGeom{d.n_layer, d.n_head_kv, d.head_dim, d.page_size, d.max_pages, (size_t)page_elems};
     const size_t entries = (size_t)d.max_seqs * d.max_pages, pool = (size_t)d.n_pages * page_elems * kv->elem;
     kv->pages.init(d.page_size, d.n_pages, d.max_seqs, d.max_pages);
-    const size_t part = (size_t)KV_SPLIT_CTAS * KV_SPLIT_ROWS * (d.head_dim + 2) * 4;
+    const size_t part = (size_t)KV_SPLIT_CTAS * KV_SPLIT_ROWS * (d.head_dim + 4) * 4;
     if (cudaMalloc(&kv->pool, pool) != cudaSuccess || cudaMalloc((void**)&kv->table, entries * 4) != cudaSuccess ||
         cudaMalloc((void**)&kv->lens, (size_t)d.max_seqs * 8) != cudaSuccess || cudaMalloc((void**)&kv->part, part) != cudaSuccess ||
         cudaMalloc((void**)&kv->tickets, KV_SPLIT_CTAS * 4) != cudaSuccess) {
