@@ -435,18 +435,18 @@ static int launch_many(const AttnArgs& a, uint32_t tiles) {
     return launch_attn(k_attn_many<T, HD, RG, KH>, set, a, tiles, RG * KH * 32, Many<T, HD, RG, KH>::SMEM, false);
 }
 template <typename T, int HD>
-static int launch_rows(const AttnArgs& a, uint32_t rows, uint32_t tiles) {
+static int launch_rows(const AttnArgs& a, const KvCache& kv, uint32_t rows, uint32_t tiles) {
     if constexpr (HD == 32 && sizeof(T) == 2) if (rows == 128) return launch_many<T, HD, 8, 1>(a, tiles);
-    if (rows == 128) return launch_attn_tc(a, tiles);
+    if (rows == 128) return launch_attn_tc(a, kv, tiles);
     return rows == 64 ? launch_many<T, HD, 4, 2>(a, tiles) : rows == 32 ? launch_many<T, HD, 2, 4>(a, tiles) : launch_few<T, HD>(a, tiles);
 }
 template <typename T>
-static int launch_hd(const AttnArgs& a, uint32_t rows, uint32_t tiles) {
+static int launch_hd(const AttnArgs& a, const KvCache& kv, uint32_t rows, uint32_t tiles) {
     switch (a.geo.hd) {
-    case 32: return launch_rows<T, 32>(a, rows, tiles);
-    case 64: return launch_rows<T, 64>(a, rows, tiles);
-    case 128: return launch_rows<T, 128>(a, rows, tiles);
-    default: return launch_rows<T, 256>(a, rows, tiles);
+    case 32: return launch_rows<T, 32>(a, kv, rows, tiles);
+    case 64: return launch_rows<T, 64>(a, kv, rows, tiles);
+    case 128: return launch_rows<T, 128>(a, kv, rows, tiles);
+    default: return launch_rows<T, 256>(a, kv, rows, tiles);
     }
 }
 
@@ -474,6 +474,7 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     a.window = window >= 1u << 30 ? 0u : window;         // no sequence is that long
     a.n_sink = n_sink; a.scale = scale; a.cap = cap; a.err = g.dev_err;
     a.part = kv->part; a.tickets = kv->tickets;
+    a.pool_rows = (uint32_t)((uint64_t)kv->d.n_pages * kv->geo.page_elems / kv->d.head_dim);
     // Tiles: every entry has its rows * group / ROWS and a part of one more.
     const uint32_t entries = std::min(n_seqs, n_rows), sms = (uint32_t)g.sm_count;
     const uint64_t flat = (uint64_t)n_rows * a.group;
@@ -499,7 +500,7 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
         while (c < a.splits && c < FEW_CLUSTER) c *= 2;
         if (a.splits <= FEW_CLUSTER || (getenv("AT_CL"))) a.splits = c;
     }
-    const int rc = kv->elem == 2 ? launch_hd<__half>(a, rows, tiles) : launch_hd<float>(a, rows, tiles);
+    const int rc = kv->elem == 2 ? launch_hd<__half>(a, *kv, rows, tiles) : launch_hd<float>(a, *kv, rows, tiles);
     end_of_op();
     return rc;
 }

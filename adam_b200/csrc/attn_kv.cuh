@@ -12,6 +12,7 @@ struct AttnArgs {
     float scale, cap;
     uint32_t splits, least;                             // CTAs that may share a tile's positions; chunks that one takes at least
     float* part; unsigned int* tickets;
+    uint32_t pool_rows;                                 // positions of all planes of the pool
     uint32_t* err;
 };
 
@@ -317,6 +318,6 @@ __device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, 
 
 
 // The tcgen05 form, 128 rows to a tile, over an fp16 cache with heads of 64 or 128 (attn_kv_tc.cu).
-int launch_attn_tc(const AttnArgs& a, uint32_t tiles);
+int launch_attn_tc(const AttnArgs& a, const KvCache& kv, uint32_t tiles);
 
 }  // namespace ab

@@ -13,6 +13,8 @@
 #include "attn_kv.cuh"
 #include "gemv_mma.cuh"
 
+#include <type_traits>
+
 namespace ab {
 
 constexpr int TC_ROWS = 128, TC_CB = 128, TC_THREADS = 384, TC_LOADERS = 96;
@@ -60,19 +62,21 @@ __device__ __forceinline__ bool atc_try(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void atc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void atc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void atc_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// 32 consecutive columns of this thread's lane (valid after atc_ld_wait), 16 to them
-__device__ __forceinline__ void atc_ld32(uint32_t t, float (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
-                   "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]),
-                   "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+// 16 consecutive columns of this thread's lane, valid after atc_ld_wait (through which the values pass, so that nothing is
+// computed from them ahead of it); 8 to them
+__device__ __forceinline__ void atc_ld16(uint32_t t, float (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
                  : "r"(t) : "memory");
 }
-__device__ __forceinline__ void atc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void atc_st16(uint32_t t, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+__device__ __forceinline__ void atc_ld_wait(float (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :: "memory");
+}
+__device__ __forceinline__ void atc_st8(uint32_t t, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void atc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float atc_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -80,15 +84,15 @@ __device__ __forceinline__ float atc_exp2(float x) { float y; asm("ex2.approx.ft
 // Columns of tensor memory: S / P of the even chunks, of the odd ones, then O' of each
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
-template <int HD>
-__global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ AttnArgs a) {
+template <int HD, bool TMA, bool CAP>
+__global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map, uint32_t run) {
     using F = AttnTc<HD>;
     extern __shared__ uint8_t raw[];
     __shared__ AttnRow s_row[TC_ROWS];
     __shared__ float s_unit[TC_ROWS];
     __shared__ uint32_t s_tmem, s_dead;
     __shared__ Found s_found;
-    __shared__ int64_t s_where[2][TC_CB];
+    __shared__ int64_t s_where[2][TMA ? 1 : TC_CB];
     __shared__ End<TC_ROWS, 2> s_end;
     // chunk c, stage c & 1: its keys are there / its scores are (and its keys read); its values / its weights / its output (and its values read)
     __shared__ __align__(8) uint64_t b_k[2], b_s[2], b_v[2], b_p[2], b_o[2];
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     uint8_t* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const uint32_t sm_s = smem_u32(sm);
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], TC_LOADERS); mbar_init(&b_s[i], 1); mbar_init(&b_v[i], TC_LOADERS); mbar_init(&b_p[i], 128); mbar_init(&b_o[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], TMA ? 1 : TC_LOADERS); mbar_init(&b_s[i], 1); mbar_init(&b_v[i], TMA ? 1 : TC_LOADERS); mbar_init(&b_p[i], 128); mbar_init(&b_o[i], 1); }
         s_dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -155,8 +159,39 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp < 11) {
-            // ---- keys and values ----
+        if (TMA && warp == 8) {
+            // ---- keys and values, a run of positions of one page to a copy; the swizzle is the copy's ----
+            const uint32_t runs = TC_CB / run;
+            const int32_t outside = (int32_t)(a.pool_rows);      // no row of the pool: a copy from there brings zeros
+            auto locate = [&](int c) -> int32_t {
+                if (c >= n || (uint32_t)lane >= runs) return outside;
+                const int32_t p = chunk_at<TC_CB>(x, c0 + c) + lane * (int32_t)run;
+                if (p > x.hi || (p + (int32_t)run <= x.from && (uint32_t)p >= a.n_sink)) return outside;
+                const int32_t page = x.pages[(uint32_t)p / a.geo.page];
+                return page < 0 ? outside : (int32_t)(kv_index(a.geo, (uint32_t)page, a.layer, 0, kvh, (uint32_t)p % a.geo.page) / HD);
+            };
+            const int32_t v_row = (int32_t)(a.geo.n_kv * a.geo.page);
+            int32_t row = locate(0);
+            auto fetch = [&](int c, int32_t y, uint32_t base, uint64_t* free, uint64_t* full) {
+                if (c >= 2) wait(free, (uint32_t)((c >> 1) - 1) & 1u);
+                if (lane == 0) mbar_expect_tx(full, F::PLANE);
+                __syncwarp();
+                if ((uint32_t)lane < runs)
+#pragma unroll
+                    for (int d0 = 0; d0 < HD; d0 += 64)
+                        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                                     :: "r"(sm_s + base + (uint32_t)(c & 1) * F::PLANE + (d0 >> 6) * TC_BLOCK + lane * run * 128), "l"(&map), "r"(d0), "r"(y), "r"(smem_u32(full)) : "memory");
+            };
+            for (int c = 0; c < n; ++c) {
+                const int32_t next = locate(c + 1);
+                fetch(c, row, F::K, &b_s[c & 1], &b_k[c & 1]);
+                fetch(c, row == outside ? outside : row + v_row, F::V, &b_o[c & 1], &b_v[c & 1]);
+                row = next;
+            }
+            // nothing is under way when the CTA ends, also where a wait ran out
+            for (int c = max(n - 2, 0); c < n; ++c) { mbar_wait(&b_k[c & 1], (uint32_t)(c >> 1) & 1u); mbar_wait(&b_v[c & 1], (uint32_t)(c >> 1) & 1u); }
+        } else if (!TMA && warp < 11) {
+            // ---- keys and values, 16 bytes at a time ----
             const int me = tid - 256;
             const __half* const pool = reinterpret_cast<const __half*>(a.pool);
             const size_t v_off = (size_t)a.geo.n_kv * a.geo.page * HD;
@@ -187,7 +222,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             }
             at_wait<0>();
             if (owed) announce();
-        } else if (lane == 0) {
+        } else if (warp == 11 && lane == 0) {
             // ---- products: S of chunk c + 1 goes ahead of O' of chunk c ----
             auto scores = [&](int c) {
                 const int b = c & 1;
@@ -214,7 +249,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
                 for (int pass = 0; pass < 2; ++pass)
 #pragma unroll
                     for (int k = 0; k < TC_CB / 16; ++k)
-                        atc_mma_ts(tmem + COL_O + b * HD, tmem + COL_S + b * 128 + (k >> 1) * 32 + (1 - pass) * 16 + (k & 1) * 8,
+                        atc_mma_ts(tmem + COL_O + b * HD, tmem + COL_S + b * 128 + k * 16 + (1 - pass) * 8,
                                    tc_desc(sm_s + F::V + b * F::PLANE + k * 2048, TC_BLOCK, 1024), ATC_IDESC<HD, true>, pass + k > 0);
                 atc_commit(&b_o[b]);
             };
@@ -232,77 +267,87 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         const int w = warp >> 2, r = tid & 127;
         const uint32_t col = tmem + ((uint32_t)(warp & 3) << 21), s_col = col + COL_S + w * 128, o_col = col + COL_O + w * HD;
         const int32_t pos = s_row[r].pos;
-        const float unit = s_unit[r] * fabsf(a.scale), k2 = unit * 1.4426950408889634f;      // scores to powers of two
-        const float rcap = a.cap > 0.f ? __frcp_rn(a.cap) : 0.f, cap2 = a.cap * 1.4426950408889634f;
+        // scores to powers of two: times k2, or cap2 tanh of them times k2
+        const float unit = s_unit[r] * fabsf(a.scale), k2 = CAP ? unit * __frcp_rn(a.cap) : unit * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f;
         float o[HD], m = -INFINITY, l = 0.f, alpha = 0.f;
 #pragma unroll
         for (int d = 0; d < HD; ++d) o[d] = 0.f;
-        auto collect = [&](int c) {                          // O' of chunk c, which is relative to m
+        auto collect = [&](int c, float factor) {            // O' of chunk c to the outputs before it, times `factor`
             wait(&b_o[w], (uint32_t)(c >> 1) & 1u);
             atc_fence_after();
+            float v[2][16];
+            atc_ld16(o_col, v[0]);
 #pragma unroll
-            for (int d0 = 0; d0 < HD; d0 += 32) {
-                float v[32];
-                atc_ld32(o_col + d0, v);
-                atc_ld_wait();
+            for (int d0 = 0; d0 < HD; d0 += 16) {
+                float (&u)[16] = v[d0 / 16 & 1];
+                atc_ld_wait(u);
+                if (d0 + 16 < HD) atc_ld16(o_col + d0 + 16, v[(d0 / 16 + 1) & 1]);
 #pragma unroll
-                for (int d = 0; d < 32; ++d) o[d0 + d] = fmaf(o[d0 + d], alpha, v[d]);
+                for (int d = 0; d < 16; ++d) o[d0 + d] = fmaf(o[d0 + d], factor, u[d]);
             }
         };
         for (int c = w; c < n; c += 2) {
-            if (c >= 2) collect(c - 2);
             const int32_t p0 = chunk_at<TC_CB>(x, c0 + c);
             const bool all = tile_sees(a, x, p0, TC_CB);
             // position p0 + j is seen for j <= j1 and (j > j0 or j < js)
             const int32_t j1 = pos - p0, j0 = a.window ? j1 - (int32_t)a.window : -1, js = (int32_t)min(a.n_sink, 0x40000000u) - p0;
+            auto seen = [&](int j) { return j <= j1 && (j > j0 || j < js); };
             wait(&b_s[w], (uint32_t)(c >> 1) & 1u);
             atc_fence_after();
-            float mx = -INFINITY;
+            // Two turns over the scores, 16 columns at a time with the next ones under way: the maximum, the weights.  Loops of two
+            // steps, one for chunks that every row sees whole, one for the others: unrolled with every choice inside, the turns took
+            // 5500 cycles, most of them fetching instructions.
+            constexpr int STEP = 16;
+            float v[2][STEP], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+            atc_ld16(s_col, v[0]);
+            auto maximum = [&](auto whole) {
 #pragma unroll 1
-            for (int d0 = 0; d0 < TC_CB; d0 += 32) {
-                float v[32];
-                atc_ld32(s_col + d0, v);
-                atc_ld_wait();
-                if (all) {
+                for (int i = 0; i < TC_CB; i += 2 * STEP)
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) mx = fmaxf(mx, v[d]);
-                } else {
+                    for (int h = 0; h < 2; ++h) {
+                        atc_ld_wait(v[h]);
+                        atc_ld16(s_col + (i + (h + 1) * STEP) % TC_CB, v[1 - h]);
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) mx = fmaxf(mx, d0 + d <= j1 && (d0 + d > j0 || d0 + d < js) ? v[d] : -INFINITY);
-                }
-            }
-            mx = a.cap > 0.f ? cap2 * at_tanh(mx * (unit * rcap)) : mx * k2;
-            const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn, shift = 8.f - ref;       // times 256: the low terms stay clear of the subnormals
+                        for (int d = 0; d < STEP; ++d) mx[d & 3] = fmaxf(mx[d & 3], decltype(whole)::value || seen(i + h * STEP + d) ? v[h][d] : -INFINITY);
+                    }
+            };
+            if (all) maximum(std::true_type{});
+            else maximum(std::false_type{});
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            top = CAP ? cap2 * at_tanh(top * k2) : top * k2;
+            const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, shift = 8.f - ref;      // times 256: the low terms stay clear of the subnormals
+            const float before = alpha;
             alpha = atc_exp2(m - ref);
             m = mn;
-            float sum = 0.f;
+            auto turn = [&](auto whole) {
 #pragma unroll 1
-            for (int d0 = 0; d0 < TC_CB; d0 += 32) {
-                float v[32];
-                atc_ld32(s_col + d0, v);
-                atc_ld_wait();
-                if (a.cap > 0.f) {
+                for (int i = 0; i < TC_CB; i += 2 * STEP)
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) v[d] = atc_exp2(fmaf(at_tanh(v[d] * (unit * rcap)), cap2, shift));
-                } else {
+                    for (int h = 0; h < 2; ++h) {
+                        float (&u)[STEP] = v[h];
+                        atc_ld_wait(u);
+                        if (i + h * STEP + STEP < TC_CB) atc_ld16(s_col + i + (h + 1) * STEP, v[1 - h]);
+                        uint32_t hi[STEP / 2], lo[STEP / 2];
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) v[d] = atc_exp2(fmaf(v[d], k2, shift));
-                }
-                if (!all)
+                        for (int d = 0; d < STEP; ++d) {
+                            u[d] = atc_exp2(CAP ? fmaf(at_tanh(u[d] * k2), cap2, shift) : fmaf(u[d], k2, shift));
+                            if (!decltype(whole)::value && !seen(i + h * STEP + d)) u[d] = 0.f;
+                        }
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) if (!(d0 + d <= j1 && (d0 + d > j0 || d0 + d < js))) v[d] = 0.f;
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int d = 0; d < 16; ++d) { sum += v[2 * d] + v[2 * d + 1]; at_split_h(v[2 * d], v[2 * d + 1], hi[d], lo[d]); }
-                atc_st16(s_col + d0, hi);
-                atc_st16(s_col + d0 + 16, lo);
-            }
-            l = fmaf(l, alpha, sum);
+                        for (int d = 0; d < STEP / 2; ++d) { sum[d & 3] += u[2 * d] + u[2 * d + 1]; at_split_h(u[2 * d], u[2 * d + 1], hi[d], lo[d]); }
+                        atc_st8(s_col + i + h * STEP, hi);
+                        atc_st8(s_col + i + h * STEP + 8, lo);
+                    }
+            };
+            if (all) turn(std::true_type{});
+            else turn(std::false_type{});
+            l = fmaf(l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (c >= 2) collect(c - 2, before);              // its products ran meanwhile; O' is free for this chunk's
             atc_st_wait();
             atc_fence_before();
             atc_arrive(&b_p[w]);
         }
-        if (n > w) collect((n - 1 - w) / 2 * 2 + w);
+        if (n > w) collect((n - 1 - w) / 2 * 2 + w, alpha);
         s_end.m[w][r] = m; s_end.l[w][r] = l * (1.f / 256.f);
         atc_fence_before();
         __syncthreads();                                     // all products are done, shared memory is free
@@ -318,18 +363,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     settle<__half, HD, TC_ROWS, 2, TC_THREADS, true, false>(a, x, s_row, t, kvh, split, sharers, reinterpret_cast<float*>(sm), s_end);
 }
 
-template <int HD>
-static int launch_tc(const AttnArgs& a, uint32_t tiles) {
+template <int HD, bool TMA, bool CAP>
+static int launch_tc(const AttnArgs& a, const KvCache& kv, uint32_t tiles) {
     static bool set = false;
     if (!set) {
-        if (cudaFuncSetAttribute((const void*)k_attn_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttnTc<HD>::SMEM) != cudaSuccess)
+        if (cudaFuncSetAttribute((const void*)k_attn_tc<HD, TMA, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttnTc<HD>::SMEM) != cudaSuccess)
             return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot raise the shared-memory limit");
         set = true;
     }
-    k_attn_tc<HD><<<dim3(tiles * a.splits, a.geo.n_kv), TC_THREADS, AttnTc<HD>::SMEM, g.stream>>>(a);
+    k_attn_tc<HD, TMA, CAP><<<dim3(tiles * a.splits, a.geo.n_kv), TC_THREADS, AttnTc<HD>::SMEM, g.stream>>>(a, kv.map, kv.run);
     count_launch();
     return check_launch("map_attn_kv");
 }
-int launch_attn_tc(const AttnArgs& a, uint32_t tiles) { return a.geo.hd == 64 ? launch_tc<64>(a, tiles) : launch_tc<128>(a, tiles); }
+template <int HD, bool TMA>
+static int launch_cap(const AttnArgs& a, const KvCache& kv, uint32_t tiles) {
+    return a.cap > 0.f ? launch_tc<HD, TMA, true>(a, kv, tiles) : launch_tc<HD, TMA, false>(a, kv, tiles);
+}
+int launch_attn_tc(const AttnArgs& a, const KvCache& kv, uint32_t tiles) {
+    if (kv.run) return a.geo.hd == 64 ? launch_cap<64, true>(a, kv, tiles) : launch_cap<128, true>(a, kv, tiles);
+    return a.geo.hd == 64 ? launch_cap<64, false>(a, kv, tiles) : launch_cap<128, false>(a, kv, tiles);
+}
 
 }  // namespace ab

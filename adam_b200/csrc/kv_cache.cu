@@ -109,6 +109,24 @@ void kv_destroy_all() {
     for (KvCache*& kv : g_kv) if (kv) { release(kv); kv = nullptr; }
 }
 
+// The pool for the tensor copies of attn_kv_tc.cu, where a page's positions come in groups of eight (the swizzle's period).
+static int make_map(KvCache& kv) {
+    const adam_b200_kv_desc& d = kv.d;
+    const uint64_t rows = (uint64_t)d.n_pages * kv.geo.page_elems / d.head_dim;
+    if (!d.kv_dtype || (d.head_dim != 64 && d.head_dim != 128) || d.page_size % 8 || rows >= (1ull << 31) - 256) return ADAMAH_OK;
+    kv.run = 8;
+    while (kv.run < 128 && d.page_size % (2 * kv.run) == 0) kv.run *= 2;
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &found) != cudaSuccess || !entry)
+        return fail(ADAMAH_ERR_BACKEND, "kv_create: the driver has no tensor maps");
+    const cuuint64_t dims[2] = {d.head_dim, rows}, strides[1] = {(cuuint64_t)d.head_dim * 2};
+    const cuuint32_t box[2] = {64, kv.run}, step[2] = {1, 1};
+    const CUresult rc = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(entry)(&kv.map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, kv.pool, dims, strides, box, step,
+        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? ADAMAH_OK : fail(ADAMAH_ERR_BACKEND, "kv_create: no tensor map (%d)", (int)rc);
+}
+
 static int create(const adam_b200_kv_desc& desc, uint32_t id) {
     adam_b200_kv_desc d = desc;
     if (d.page_size == 0) d.page_size = 64;
@@ -139,6 +157,7 @@ static int create(const adam_b200_kv_desc& desc, uint32_t id) {
         cudaMemsetAsync(kv->lens, 0, (size_t)d.max_seqs * 8, g.stream) != cudaSuccess || cudaMemsetAsync(kv->tickets, 0, KV_SPLIT_CTAS * 4, g.stream) != cudaSuccess ||
         cudaStreamSynchronize(g.stream) != cudaSuccess)
         return fail(ADAMAH_ERR_BACKEND, "kv_create: %s", cudaGetErrorString(cudaGetLastError()));
+    if (int rc = make_map(*kv)) return rc;
     g_kv[id] = kv;
     guard.kv = nullptr;
     return ADAMAH_OK;

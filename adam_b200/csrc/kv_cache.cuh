@@ -4,6 +4,8 @@
 #include "kv_pages.h"
 #include "token.cuh"
 
+#include <cuda.h>
+
 namespace ab {
 
 constexpr uint32_t MAX_KV = 64;
@@ -21,6 +23,8 @@ struct KvCache {
     int32_t* own_from;                   // [max_seqs] first position that the sequence may write (those before may be others', too)
     float* part;                         // partial results of attention CTAs that share a tile's positions
     unsigned int* tickets;               // arrivals per tile, zero between calls
+    CUtensorMap map;                     // the pool as rows of head_dim fp16 values, in boxes of `run` rows of 64 (run = 0: none)
+    uint32_t run;                        // positions of a page that a box holds
     KvPages pages;                       // the same on the host, where pages are given out
 };
 
