@@ -4,8 +4,8 @@
 //   s_j = scale q.k_j, or cap tanh(scale q.k_j / cap);   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   j visible to the row
 //
 // The rows of an entry times the query heads of a key head are one list, cut into tiles that share what they read of the
-// cache.  Both products run on the tensor cores with the operands at the precision of 32 bits: the cache's fp16 values are
-// exact operands, and a query row or a row of weights goes in as two fp16 terms (22 bits); a float32 cache takes three tf32
+// cache: 2 or 4 rows in 32-bit arithmetic (attn_kv_thin.cu), 128 by tcgen05 (attn_kv_tc.cu), the widths between them here.  On
+// the tensor cores both products have operands at the precision of 32 bits: the cache's fp16 values are exact operands, and a query row or a row of weights goes in as two fp16 terms (22 bits); a float32 cache takes three tf32
 // products (x_hi y_hi + x_hi y_lo + x_lo y_hi).  A chunk's P V goes into fresh accumulators and joins the running output in
 // fp32 with the rescaling that the running maximum needs anyway: the tensor core rounds its sums towards zero, and a sum
 // over 65000 positions that never left it would be 2e-4 off.
@@ -16,7 +16,6 @@
 #include "attn_kv.cuh"
 
 #include <algorithm>
-#include <cstdlib>
 
 namespace ab {
 
@@ -195,7 +194,7 @@ __device__ __forceinline__ void values_f(float (&o)[HD / 8][4], const float (&s)
 
 // The warps' results into shared memory, then the rest of the way.
 template <typename T, int HD, int ROWS, int PLANES, int THREADS, bool CLUSTER>
-__device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
+__device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, const AttnShare& part, uint32_t sharers,
                                        int plane, int r0, const float (&o)[HD / 8][4], const float (&m)[2], float (&l)[2], float* merge, End<ROWS, PLANES>& end) {
     constexpr int LM = HD + 4;
     constexpr float UNIT = sizeof(T) == 2 ? 1.f / 256.f : 1.f;
@@ -215,13 +214,12 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const AttnTile& x, con
         for (int j = 0; j < HD / 8; ++j)
             *reinterpret_cast<float2*>(merge + (plane * ROWS + r) * LM + 8 * j + 2 * q4) = make_float2(o[j][2 * h] * f, o[j][2 * h + 1] * f);
     }
-    settle<T, HD, ROWS, PLANES, THREADS, false, CLUSTER>(a, x, rows, t, kvh, split, sharers, merge, end);
+    settle<T, HD, ROWS, PLANES, THREADS, false, CLUSTER>(a, x, rows, part, sharers, merge, end);
 }
 // ---- few rows: 16 per tile -------------------------------------------------------------------------------------------
 // Every warp has chunks of 16 positions of its own (chunk w, w + W, ..), the next ones under way in STAGES slots of
-// shared memory, and its own running maxima, sums and outputs; nothing in the loop waits for another warp.  Bound by HBM: the tensor
-// cores are busy for a few percent.
-constexpr uint32_t FEW_CLUSTER = 16;                 // CTAs that share a tile as a cluster, at most
+// shared memory, and its own running maxima, sums and outputs; nothing in the loop waits for another warp.  Bound by what a warp
+// has to do in turn for a chunk of 16 positions, most of it for rows that a tile may not have.
 template <typename T, int HD>
 struct Few {
     static constexpr int ROWS = 16, CB = 16, ROW_BYTES = HD * (int)sizeof(T);
@@ -246,11 +244,12 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
     __shared__ Found s_found;
     __shared__ End<ROWS, W> s_end;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
-    const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = blockIdx.x / a.splits;
+    const AttnShare part = share_of(a);
+    const uint32_t kvh = part.kvh;
     AttnTile x;
-    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_found)) return;
+    if (!find_tile<ROWS, CB>(a, part.tile, kvh, x, s_row, s_found)) return;
     uint32_t sharers, c0, c1;
-    if (!share_out(a, x, split, sharers, c0, c1) && !CLUSTER) return;         // in a cluster it still takes its rows
+    if (!share_out(a, x, part, sharers, c0, c1) && !CLUSTER) return;         // in a cluster it still takes its rows
     c0 = min(c0, c1);
 
     uint8_t* const ring = sm + F::Q_BYTES + warp * STAGES * F::SLOT;
@@ -311,10 +310,10 @@ __global__ void __launch_bounds__(Few<T, HD>::W * 32) k_attn_few(const __grid_co
         slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     at_wait<0>();
-    finish<T, HD, ROWS, W, W * 32, CLUSTER>(a, x, s_row, t, kvh, split, sharers, warp, 0, o, m, l, reinterpret_cast<float*>(sm + F::Q_BYTES), s_end);
+    finish<T, HD, ROWS, W, W * 32, CLUSTER>(a, x, s_row, part, sharers, warp, 0, o, m, l, reinterpret_cast<float*>(sm + F::Q_BYTES), s_end);
 }
 
-// ---- many rows: 32 to 128 per tile -----------------------------------------------------------------------------------
+// ---- many rows: 32 or 64 per tile ------------------------------------------------------------------------------------
 // RG groups of 16 rows, KH warps to a group, each with its share of every chunk's positions; two chunks of keys and values in
 // shared memory for all of them.
 template <typename T, int HD, int RG, int KH>
@@ -338,11 +337,12 @@ __global__ void __launch_bounds__(RG * KH * 32) k_attn_many(const __grid_constan
     __shared__ int64_t s_where[2][CB];
     __shared__ End<ROWS, KH> s_end;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rg = warp % RG, kh = warp / RG, r0 = rg * 16, g = lane >> 2;
-    const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = blockIdx.x / a.splits;
+    const AttnShare part = share_of(a);
+    const uint32_t kvh = part.kvh;
     AttnTile x;
-    if (!find_tile<ROWS, CB>(a, t, kvh, x, s_row, s_found)) return;
+    if (!find_tile<ROWS, CB>(a, part.tile, kvh, x, s_row, s_found)) return;
     uint32_t sharers, c0, c1;
-    if (!share_out(a, x, split, sharers, c0, c1)) return;
+    if (!share_out(a, x, part, sharers, c0, c1)) return;
     uint8_t* const tiles = sm + F::Q_BYTES;              // chunk c: keys at (c & 1) * 2 PART, values behind them
     const uint32_t tiles_s = at_smem(tiles), q_s = at_smem(sm);
     const T* const pool = reinterpret_cast<const T*>(a.pool);
@@ -405,48 +405,36 @@ __global__ void __launch_bounds__(RG * KH * 32) k_attn_many(const __grid_constan
         request(c + 2);
     }
     at_wait<0>();
-    finish<T, HD, ROWS, KH, THREADS, false>(a, x, s_row, t, kvh, split, sharers, kh, r0, o, m, l, reinterpret_cast<float*>(sm), s_end);
+    finish<T, HD, ROWS, KH, THREADS, false>(a, x, s_row, part, sharers, kh, r0, o, m, l, reinterpret_cast<float*>(sm), s_end);
 }
 
-template <typename K>
-static int launch_attn(K kernel, bool& set, const AttnArgs& a, uint32_t tiles, int threads, int smem, bool cluster) {
-    if (!set) {
-        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            (cluster && cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
-            return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot set the kernel's limits");
-        set = true;
-    }
-    const dim3 grid(tiles * a.splits, a.geo.n_kv);
-    if (cluster) launch_k_cluster(kernel, grid, dim3(threads), smem, g.stream, false, a.splits, false, a);
-    else kernel<<<grid, threads, smem, g.stream>>>(a);
-    count_launch();
-    return check_launch("map_attn_kv");
-}
 template <typename T, int HD>
-static int launch_few(const AttnArgs& a, uint32_t tiles) {
+static int launch_few(const AttnArgs& a) {
     static bool set[2] = {false, false};
     using F = Few<T, HD>;
-    if (a.splits > 1 && a.splits <= FEW_CLUSTER) return launch_attn(k_attn_few<T, HD, true>, set[1], a, tiles, F::W * 32, F::SMEM, true);
-    return launch_attn(k_attn_few<T, HD, false>, set[0], a, tiles, F::W * 32, F::SMEM, false);
+    if (attn_cluster(a)) return launch_attn(k_attn_few<T, HD, true>, set[1], a, F::W * 32, F::SMEM, true);
+    return launch_attn(k_attn_few<T, HD, false>, set[0], a, F::W * 32, F::SMEM, false);
 }
 template <typename T, int HD, int RG, int KH>
-static int launch_many(const AttnArgs& a, uint32_t tiles) {
+static int launch_many(const AttnArgs& a) {
     static bool set = false;
-    return launch_attn(k_attn_many<T, HD, RG, KH>, set, a, tiles, RG * KH * 32, Many<T, HD, RG, KH>::SMEM, false);
+    return launch_attn(k_attn_many<T, HD, RG, KH>, set, a, RG * KH * 32, Many<T, HD, RG, KH>::SMEM, false);
 }
 template <typename T, int HD>
-static int launch_rows(const AttnArgs& a, const KvCache& kv, uint32_t rows, uint32_t tiles) {
-    if constexpr (HD == 32 && sizeof(T) == 2) if (rows == 128) return launch_many<T, HD, 8, 1>(a, tiles);
-    if (rows == 128) return launch_attn_tc(a, kv, tiles);
-    return rows == 64 ? launch_many<T, HD, 4, 2>(a, tiles) : rows == 32 ? launch_many<T, HD, 2, 4>(a, tiles) : launch_few<T, HD>(a, tiles);
+static int launch_rows(const AttnArgs& a, const KvCache& kv, uint32_t rows) {
+    if (rows <= 4) return launch_attn_thin(a, sizeof(T), rows);
+    if (rows == 16) return launch_few<T, HD>(a);
+    // 32 and 64: the only choice for heads of 256, and floats of 128
+    if constexpr (HD == 256 || (HD == 128 && sizeof(T) == 4)) return rows == 64 ? launch_many<T, HD, 4, 2>(a) : launch_many<T, HD, 2, 4>(a);
+    else return launch_attn_tc(a, kv);
 }
 template <typename T>
-static int launch_hd(const AttnArgs& a, const KvCache& kv, uint32_t rows, uint32_t tiles) {
+static int launch_hd(const AttnArgs& a, const KvCache& kv, uint32_t rows) {
     switch (a.geo.hd) {
-    case 32: return launch_rows<T, 32>(a, kv, rows, tiles);
-    case 64: return launch_rows<T, 64>(a, kv, rows, tiles);
-    case 128: return launch_rows<T, 128>(a, kv, rows, tiles);
-    default: return launch_rows<T, 256>(a, kv, rows, tiles);
+    case 32: return launch_rows<T, 32>(a, kv, rows);
+    case 64: return launch_rows<T, 64>(a, kv, rows);
+    case 128: return launch_rows<T, 128>(a, kv, rows);
+    default: return launch_rows<T, 256>(a, kv, rows);
     }
 }
 
@@ -479,28 +467,54 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     const uint32_t entries = std::min(n_seqs, n_rows), sms = (uint32_t)g.sm_count;
     const uint64_t flat = (uint64_t)n_rows * a.group;
     auto tiles_of = [&](uint64_t rows) { return (flat + (rows - 1) * entries) / rows; };
-    if (tiles_of(16) * a.geo.n_kv >= (1u << 30)) return fail(ADAMAH_ERR_INVALID, "attn_kv: %u rows of %u heads", n_rows, n_head);
-    // Rows of a tile: 16 where the entries have no more, else the widest whose tiles still give every SM one.  A wide tile reads
-    // the cache less often; below one tile per SM the time is that of the longest tile.
-    uint32_t rows = 16;
-    if (flat > 16ull * entries)
-        for (rows = kv->elem == 2 && a.geo.hd <= 128 ? 128 : 64; rows > 32; rows /= 2)
-            if (flat / rows * a.geo.n_kv >= sms) break;
-    if (getenv("AT_ROWS")) rows = atoi(getenv("AT_ROWS"));
-    const uint32_t tiles = (uint32_t)tiles_of(rows), ctas = tiles * a.geo.n_kv;
-    // Splits: as many CTAs as the GPU holds at once, no more than the workspace has room for.  How far the sequences reach
-    // only decides the launch; a graph that is replayed later divides what there is then.
+    if (tiles_of(2) * a.geo.n_kv >= (1u << 30)) return fail(ADAMAH_ERR_INVALID, "attn_kv: %u rows of %u heads", n_rows, n_head);
+    // How far the sequences reach only decides the launch; a graph that is replayed later divides what there is then.
     uint32_t reach = kv->pages.longest();
     if (a.window) reach = (uint32_t)std::min<uint64_t>(reach, (uint64_t)a.window + n_sink);
-    const uint32_t chunk = rows == 16 ? 16 : rows == 128 && a.geo.hd > 32 ? 128 : kv->elem == 2 ? 64 : 32;
+    const uint32_t parts = (reach + 127) / 128, hd = a.geo.hd;
+    const bool f16 = kv->elem == 2;
+    const uint32_t rows = [&]() -> uint32_t {
+        // Rows of a tile.  The measured times are of 32 heads over 16 of 128 dims if not said otherwise, fp16 cache.
+        const uint64_t work16 = tiles_of(16) * a.geo.n_kv * parts, work64 = tiles_of(64) * a.geo.n_kv * parts;
+        // 2 or 4 in 32-bit arithmetic where an entry has no more (64 decoding sequences of 2047: 125 us against 205 in tiles of 16).
+        // Over floats, whose tensor-core products come in threes, also for more: 8 sequences of 16 new tokens behind 1000: 92 us against
+        // 139; with heads of 256 until the whole is large: one of 64 behind 8000, 4 heads over 1: 125 us against 121 to 183.  With
+        // fp16 heads of 256 while the whole is small: 8 tokens behind 8000, 4 heads over 1: 33 us against 55.
+        const bool thin = f16 ? flat <= 4ull * entries || (hd == 256 && work16 <= 2ull * sms) : flat <= 32ull * entries || (hd == 256 && work64 <= 16ull * sms);
+        if (thin && a.geo.page % attn_thin_chunk(kv->elem, hd) == 0) return flat <= 2ull * entries ? 2 : 4;
+        // 16 where an entry has no more (wider tiles would be empty: 32 entries of 8 tokens behind 1000: 67 us against 85), where the whole is
+        // small, so that more CTAs count for more than less reading (16 tokens behind 2000: 20 us against 22; behind 8000 and 64 tokens: 121
+        // against 50), and for short rows, where the wider tiles never won.
+        if (flat <= 16ull * entries || work16 <= 7ull * sms || hd * kv->elem <= 64 || (!f16 && hd == 64)) return 16;
+        if (f16 && hd <= 128) return 128;
+        // 64 for a large whole (1024 tokens behind 8000, heads of 256, 4 over 1: 333 us against 447; 2048 tokens of a prompt: 156 against 115)
+        return work64 > 16ull * sms ? 64 : 32;
+    }();
+    a.pairs = (uint32_t)tiles_of(rows) * a.geo.n_kv;
+    // Splits: what fills the GPU once and again is left whole, and the rest (or all, where it is less) divided among as many CTAs
+    // as the GPU holds at once, no more than the workspace has room for: 512 tiles on 148 SMs take 3.5 turns, not 4.
+    const uint32_t chunk = rows <= 4 ? attn_thin_chunk(kv->elem, hd) : rows == 16 ? 16 : rows == 128 ? 128 : f16 ? 64 : 32;
     a.least = 128 / chunk;
-    a.splits = std::max(1u, std::min({sms * (rows == 16 ? 2 : 1) / ctas, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / ctas, (reach + 127) / 128}));
-    if (rows == 16 && a.splits > 1) {                    // a cluster where that is enough: 2, 4, 8 or 16 of them
-        uint32_t c = 1;
-        while (c < a.splits && c < FEW_CLUSTER) c *= 2;
-        if (a.splits <= FEW_CLUSTER || (getenv("AT_CL"))) a.splits = c;
+    const uint32_t slots = sms * (rows <= 4 ? THIN_CTAS : rows == 16 ? 2 : 1), rest = a.pairs % slots;
+    a.whole = a.pairs; a.splits = 1;
+    if (rest) {
+        a.splits = std::min({slots / rest, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / rest, parts});
+        // The last CTA adds up 128 rows of each: no more of them than the square root of twice the parts (8 heads over 1, 8 tokens
+        // behind 8000: 71 us with 63 splits, 32 with 11)
+        if (rows == 128)
+            for (uint32_t most = 1; most < a.splits; ++most)
+                if (most * most >= 2 * parts) a.splits = most;
+        // Clusters of 2, 4 or 8 where that is about enough, or of 16 as long as they find their place (16 key heads behind 2000: 17 us in
+        // 8, 24 in 16).  What a power of two leaves idle counts for long sequences.
+        if (rows <= 16 && rest == a.pairs && a.splits <= ATTN_CLUSTER) {
+            uint32_t c = 1;
+            while (2 * c <= a.splits && (c < 8 || 16 * rest <= sms)) c *= 2;
+            if (4 * c >= 3 * a.splits || reach < 1024 * a.splits) a.splits = c;
+        }
+        if (a.splits > 1) a.whole = a.pairs - rest;
+        else a.splits = 1;
     }
-    const int rc = kv->elem == 2 ? launch_hd<__half>(a, *kv, rows, tiles) : launch_hd<float>(a, *kv, rows, tiles);
+    const int rc = kv->elem == 2 ? launch_hd<__half>(a, *kv, rows) : launch_hd<float>(a, *kv, rows);
     end_of_op();
     return rc;
 }

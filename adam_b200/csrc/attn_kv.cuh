@@ -10,7 +10,8 @@ struct AttnArgs {
     KvBatch b; KvGeom geo; const void* pool;
     uint32_t layer, n_head, group, window, n_sink;      // group: query heads of a key head
     float scale, cap;
-    uint32_t splits, least;                             // CTAs that may share a tile's positions; chunks that one takes at least
+    uint32_t pairs, whole, splits, least;               // (tile, key head)s; how many of them one CTA has alone; CTAs that may share
+                                                        // the positions of each of the others; chunks that one takes at least
     float* part; unsigned int* tickets;
     uint32_t pool_rows;                                 // positions of all planes of the pool
     uint32_t* err;
@@ -131,6 +132,26 @@ __device__ __forceinline__ void at_split_h(float x, float y, uint32_t& hi, uint3
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t*>(&h); lo = *reinterpret_cast<const uint32_t*>(&l);
 }
+// two values an instruction
+__device__ __forceinline__ float2 at_fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 at_mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 at_add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float at_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // A power of two that brings the largest of a row's values (its magnitude `most`) into [2^7, 2^8), and its inverse: fp16 terms
 // then neither overflow nor lose bits of what counts.
 __device__ __forceinline__ void row_scale(float most, float& up, float& down) {
@@ -220,9 +241,29 @@ __device__ __forceinline__ const float* of_rank(const float* p, uint32_t rank) {
 }
 __device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// What a CTA does: a tile's rows of a key head, one of `of` parts of their positions.  Tiles from the last one on: late rows see more.
+struct AttnShare { uint32_t tile, kvh, split, of, slot; };      // slot: of the shared ones, in the workspace
+__device__ __forceinline__ AttnShare share_of(const AttnArgs& a) {
+    const uint32_t b = blockIdx.x;
+    AttnShare s{0, 0, 0, 1, 0};
+    uint32_t pair = b;
+    if (b >= a.whole) { s.slot = (b - a.whole) / a.splits; s.split = (b - a.whole) % a.splits; s.of = a.splits; pair = a.whole + s.slot; }
+    const uint32_t tiles = a.pairs / a.geo.n_kv;
+    s.kvh = pair / tiles; s.tile = tiles - 1 - pair % tiles;
+    return s;
+}
+inline uint32_t attn_grid(const AttnArgs& a) { return a.whole + (a.pairs - a.whole) * a.splits; }
+// This CTA's chunks of the tile; false: it has none
+__device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, const AttnShare& s, uint32_t& sharers, uint32_t& c0, uint32_t& c1) {
+    const uint32_t each = max((x.chunks + s.of - 1) / s.of, a.least);
+    sharers = s.of > 1 ? (x.chunks + each - 1) / each : 1u;
+    c0 = s.split * each; c1 = s.of > 1 ? min(x.chunks, c0 + each) : x.chunks;
+    return s.split < sharers;
+}
+
 // By all THREADS of the CTA, m, l and merge written.  CLUSTER: the tile's CTAs (a.splits of them) are one.
 template <typename T, int HD, int ROWS, int PLANES, int THREADS, bool BASE2, bool CLUSTER>
-__device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, uint32_t t, uint32_t kvh, uint32_t split, uint32_t sharers,
+__device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, const AttnRow* rows, const AttnShare& part, uint32_t sharers,
                                        float* merge, End<ROWS, PLANES>& end) {
     using E = End<ROWS, PLANES>;
     constexpr int LM = HD + 4, VPR = HD / 4, PER = (ROWS * VPR + THREADS - 1) / THREADS;       // values in fours; of a row, of a thread
@@ -252,72 +293,114 @@ __device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, con
     if (CLUSTER && a.splits > 1) {
         for (uint32_t i = tid; i < live * VPR; i += THREADS) *reinterpret_cast<float4*>(merge + i / VPR * LM + i % VPR * 4) = value(i / VPR, i % VPR * 4);
         cluster_meet();
-        first = split; every = a.splits;
+        first = part.split; every = a.splits;
     } else if (sharers > 1) {
-        const size_t tile = (size_t)t * a.geo.n_kv + kvh, step = (size_t)ROWS * (HD + 4);      // per row: the values, the maximum, the sum
-        float* mine = a.part + (tile * a.splits + split) * step;
+        const size_t step = (size_t)ROWS * (HD + 4);     // per row: the values, the maximum, the sum
+        float* mine = a.part + ((size_t)part.slot * a.splits + part.split) * step;
         for (uint32_t i = tid; i < live * VPR; i += THREADS) *reinterpret_cast<float4*>(mine + i / VPR * LM + i % VPR * 4) = value(i / VPR, i % VPR * 4);
         for (uint32_t r = tid; r < live; r += THREADS) *reinterpret_cast<float2*>(mine + r * LM + HD) = make_float2(end.m[0][r], end.l[0][r]);
         __threadfence();
         __syncthreads();
-        if (tid == 0) end.ticket = atomicInc(a.tickets + tile, sharers - 1);
+        if (tid == 0) end.ticket = atomicInc(a.tickets + part.slot, sharers - 1);
         __syncthreads();
         if (end.ticket != sharers - 1) return;
         __threadfence();
     }
-    const float* all = a.part + ((size_t)t * a.geo.n_kv + kvh) * a.splits * ROWS * LM;
-    float4 out[PER];
-#pragma unroll
+    const float* all = a.part + (size_t)part.slot * a.splits * ROWS * LM;
+    // A few results of a thread stay in registers (also where other CTAs read the sums); more go where the sums lie, by a short loop
+    // (seven copies of it, met once by a
+    // CTA, took 5 us to fetch).
+    constexpr bool KEEP = PER <= 4 || CLUSTER;
+    float4 out[KEEP ? PER : 1];
+#pragma unroll(KEEP ? PER : 1)
     for (int j = 0; j < PER; ++j) {
         const uint32_t i = tid + j * THREADS, r = first + i / VPR * every, d = i % VPR * 4;
         if (r >= live) break;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float z = 0.f;
         if ((CLUSTER && a.splits > 1) || sharers > 1) {
+            // eight at a time, in their order, relative to the maximum so far
             float b = -INFINITY;
-            auto ml = [&](uint32_t k) {
-                if (CLUSTER) return make_float2(*of_rank(&end.m[0][r], k), *of_rank(&end.l[0][r], k));
-                return __ldcg(reinterpret_cast<const float2*>(all + ((size_t)k * ROWS + r) * LM + HD));
-            };
-#pragma unroll 4
-            for (uint32_t k = 0; k < sharers; ++k) b = max_nan(b, ml(k).x);
-#pragma unroll 4
-            for (uint32_t k = 0; k < sharers; ++k) {
-                const float2 q = ml(k);
-                const float w = E::template weight<BASE2>(q.x, b);
-                z = fmaf(q.y, w, z);
-                add(v, w, CLUSTER ? *reinterpret_cast<const float4*>(of_rank(merge + r * LM + d, k)) : __ldcg(reinterpret_cast<const float4*>(all + ((size_t)k * ROWS + r) * LM + d)));
+            constexpr uint32_t U = 8;
+#pragma unroll 1
+            for (uint32_t k0 = 0; k0 < sharers; k0 += U) {
+                float2 q[U];
+                float4 y[U];
+                float top = b;
+#pragma unroll
+                for (uint32_t k = 0; k < U; ++k) {
+                    const uint32_t c = k0 + k;
+                    q[k] = make_float2(-INFINITY, 0.f); y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c >= sharers) continue;
+                    if (CLUSTER) {
+                        q[k] = make_float2(*of_rank(&end.m[0][r], c), *of_rank(&end.l[0][r], c));
+                        y[k] = *reinterpret_cast<const float4*>(of_rank(merge + r * LM + d, c));
+                    } else {
+                        const float* from = all + ((size_t)c * ROWS + r) * LM;
+                        q[k] = __ldcg(reinterpret_cast<const float2*>(from + HD));
+                        y[k] = __ldcg(reinterpret_cast<const float4*>(from + d));
+                    }
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < U; ++k) top = max_nan(top, q[k].x);
+                const float w0 = E::template weight<BASE2>(b, top);
+                v.x *= w0; v.y *= w0; v.z *= w0; v.w *= w0; z *= w0;
+                b = top;
+#pragma unroll
+                for (uint32_t k = 0; k < U; ++k) {
+                    const float w = E::template weight<BASE2>(q[k].x, b);
+                    z = fmaf(q[k].y, w, z);
+                    add(v, w, y[k]);
+                }
             }
         } else { v = value(r, d); z = end.l[0][r]; }
-        out[j] = make_float4(v.x / z, v.y / z, v.z / z, v.w / z);
-        const float most = max_nan(max_nan(fabsf(out[j].x), fabsf(out[j].y)), max_nan(fabsf(out[j].z), fabsf(out[j].w)));
+        v = make_float4(v.x / z, v.y / z, v.z / z, v.w / z);
+        const float most = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
         if (rows[r].pos >= 0 && !(most <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
+        if constexpr (KEEP) out[j] = v;
+        else *reinterpret_cast<float4*>(merge + r * LM + d) = v;
     }
     __syncthreads();
     auto bad = [&](uint32_t r) { return end.bad[r >> 5] >> (r & 31) & 1u; };
-#pragma unroll
+#pragma unroll(KEEP ? PER : 1)
     for (int j = 0; j < PER; ++j) {
         const uint32_t i = tid + j * THREADS, r = first + i / VPR * every, d = i % VPR * 4;
         if (r >= live) break;
         if (rows[r].pos < 0 || bad(r)) continue;
         float* to = a.act + rows[r].o + d;
-        if (rows[r].o % 4 == 0) *reinterpret_cast<float4*>(to) = out[j];
-        else { to[0] = out[j].x; to[1] = out[j].y; to[2] = out[j].z; to[3] = out[j].w; }
+        float4 v;
+        if constexpr (KEEP) v = out[j];
+        else v = *reinterpret_cast<const float4*>(merge + r * LM + d);
+        if (rows[r].o % 4 == 0) *reinterpret_cast<float4*>(to) = v;
+        else { to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w; }
     }
     for (uint32_t r = first + (tid >> 5) * every; r < live; r += (THREADS >> 5) * every)
-        if (bad(r)) attend_row<T, HD>(a, x, rows[r], kvh);
+        if (bad(r)) attend_row<T, HD>(a, x, rows[r], part.kvh);
     if (CLUSTER && a.splits > 1) cluster_meet();         // nobody leaves while its shared memory is read
 }
-// This CTA's chunks of the tile; false: it has none
-__device__ __forceinline__ bool share_out(const AttnArgs& a, const AttnTile& x, uint32_t split, uint32_t& sharers, uint32_t& c0, uint32_t& c1) {
-    const uint32_t each = max((x.chunks + a.splits - 1) / a.splits, a.least);
-    sharers = (x.chunks + each - 1) / each;
-    c0 = split * each; c1 = min(x.chunks, c0 + each);
-    return split < sharers;
+// Do the CTAs that share a tile come as a cluster?  (Of tiles of 16 rows and less)
+constexpr uint32_t ATTN_CLUSTER = 16;                // at most
+inline bool attn_cluster(const AttnArgs& a) { return a.whole == 0 && a.splits > 1 && a.splits <= ATTN_CLUSTER && (a.splits & (a.splits - 1)) == 0; }
+template <typename K>
+inline int launch_attn(K kernel, bool& set, const AttnArgs& a, int threads, int smem, bool cluster) {
+    if (!set) {
+        if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            (cluster && cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
+            return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot set the kernel's limits");
+        set = true;
+    }
+    const dim3 grid(attn_grid(a));
+    if (cluster) launch_k_cluster(kernel, grid, dim3(threads), smem, g.stream, false, a.splits, false, a);
+    else kernel<<<grid, threads, smem, g.stream>>>(a);
+    count_launch();
+    return check_launch("map_attn_kv");
 }
 
-
+// Two or four rows to a tile (attn_kv_thin.cu), pages of whole chunks
+constexpr uint32_t THIN_CTAS = 3;                    // on an SM
+int launch_attn_thin(const AttnArgs& a, uint32_t elem, uint32_t rows);
+uint32_t attn_thin_chunk(uint32_t elem, uint32_t hd);
 // The tcgen05 form, 128 rows to a tile, over an fp16 cache with heads of 64 or 128 (attn_kv_tc.cu).
-int launch_attn_tc(const AttnArgs& a, const KvCache& kv, uint32_t tiles);
+int launch_attn_tc(const AttnArgs& a, const KvCache& kv);
 
 }  // namespace ab

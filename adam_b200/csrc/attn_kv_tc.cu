@@ -5,11 +5,18 @@
 //   S = (Q_hi + Q_lo) K^T    tcgen05.mma, both operands in shared memory, into 128 columns of tensor memory
 //   P = 2^(k S - m + 8)      a row to a thread: S read twice (maximum, weights), P as two fp16 terms over S, column for column
 //   O' = (P_hi + P_lo) V     tcgen05.mma, P from tensor memory, V from shared memory as it lies there (its positions are the rows)
-//   O = O alpha + O'         in registers: a sum that stays in the tensor core for many chunks would lose bits (attn_kv.cu)
-// Two warpgroups take the even and the odd chunks, each with its own S / P, O' and running maximum, so that the tensor core
-// works on one's products while the other is at its weights; they merge at the end.  Three warps fetch keys and values
-// (16 bytes at a time, so that pages may end anywhere), one thread issues the products.  Bound by the tensor core, which has two
-// products where 16-bit operands would have one; the weights need about as many cycles of the other units.
+//   O = O alpha + O' beta    in registers: a sum that stays in the tensor core for many chunks would lose bits (attn_kv.cu)
+// Two warpgroups make the weights of the even and the odd chunks, each relative to its own running maximum; two more have a half
+// of the outputs each and add up what comes relative to either.  Three S / P take turns, so that the scores of the next chunks
+// are there when a warpgroup is done with its weights (with an S / P of its own, whose scores have to wait for the output of the
+// weights before them, a warpgroup stood still for 2900 of 6700 cycles).  One warp fetches keys and another values, by tensor
+// copies, or 16 bytes at a time where pages do not come in groups of eight; one thread issues each product.
+//
+// The roles execute different code at once, and what all of them need for a chunk has to stay in an instruction cache that a few
+// SMs refill together: with loops unrolled freely it took 2600 cycles a chunk on some SMs and 4000 on others, with short ones (and
+// two values to an instruction) 2900 everywhere.  Of those the tensor core is busy for about 2700: 16 products of 64 cycles for
+// S, 16 of 107 for P V, whose first operand comes from tensor memory (107 also with half the columns).  2048 tokens behind 14000,
+// 32 heads over 16 of 128: 927 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
 #include "attn_kv.cuh"
 #include "gemv_mma.cuh"
 
@@ -17,14 +24,15 @@
 
 namespace ab {
 
-constexpr int TC_ROWS = 128, TC_CB = 128, TC_THREADS = 384, TC_LOADERS = 96;
+constexpr int TC_ROWS = 128, TC_CB = 128, TC_THREADS = 640, TC_LOADERS = 64;
+constexpr int TC_OUT = 8, TC_FETCH = 16, TC_ISSUE = 18;       // first warp of the outputs; the two that fetch; the two that issue
 constexpr uint32_t TC_BLOCK = 128 * 128;             // 128 rows (or positions) of 64 values: 128 bytes each, in the 128-byte swizzle
 
 template <int HD>
 struct AttnTc {
     static constexpr uint32_t PLANE = HD / 64 * TC_BLOCK;                       // a tile of 128 rows
     static constexpr uint32_t Q = 0, K = 2 * PLANE, V = K + 2 * PLANE, END = V + 2 * PLANE;      // two planes of Q, two stages of K and V
-    static constexpr uint32_t MERGE = 2 * TC_ROWS * (HD + 4) * 4;
+    static constexpr uint32_t MERGE = TC_ROWS * (HD + 4) * 4;
     static constexpr uint32_t SMEM = (END > MERGE ? END : MERGE) + 1024;        // + alignment
 };
 
@@ -35,9 +43,10 @@ __device__ __forceinline__ uint32_t tc_at(int r, int d) { return (uint32_t)(d >>
 // distances in 16-byte units.  Rows along M or N, values along K (Q, K): groups of 8 rows are 1024 bytes apart, the 16 values of an
 // instruction 32 bytes of a row.  The other way round (V as the second operand: N along a row, positions are K): groups of 8
 // positions 1024 bytes apart, blocks of 64 columns TC_BLOCK, the 16 positions of an instruction 2048 bytes.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// The words of a descriptor: everything but the address is known ahead, and the thread that issues products must not do more
+// than an addition for each (built anew for every product, descriptors took it 2000 cycles a chunk).
+__device__ __forceinline__ uint32_t tc_desc_lo(uint32_t addr, uint32_t leading) { return (addr & 0x3FFFFu) >> 4 | (leading >> 4) << 16; }
+__device__ __forceinline__ uint64_t tc_desc(uint32_t lo) { return (uint64_t)((1024u >> 4) | 1u << 14 | 2u << 29) << 32 | lo; }
 // kind::f16: D = f32 (1 at bit 4), A = B = f16, second operand with N along its rows (bit 16), N / 8 at bit 17, M / 16 at bit 24
 template <int N, bool N_ROWS> constexpr uint32_t ATC_IDESC = (1u << 4) | (N_ROWS ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
 
@@ -74,63 +83,87 @@ __device__ __forceinline__ void atc_ld_wait(float (&r)[16]) {
                  : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
                  :: "memory");
 }
+__device__ __forceinline__ void atc_ld8(uint32_t t, float (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]) : "r"(t) : "memory");
+}
+__device__ __forceinline__ void atc_ld_wait(float (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]) :: "memory");
+}
+__device__ __forceinline__ void atc_st4(uint32_t t, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 __device__ __forceinline__ void atc_st8(uint32_t t, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void atc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float atc_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-// Columns of tensor memory: S / P of the even chunks, of the odd ones, then O' of each
-constexpr uint32_t COL_S = 0, COL_O = 256;
+// what three roles execute for every chunk has to come out of a small instruction cache: two values an instruction, three to a maximum
+__device__ __forceinline__ float atc_max3(float a, float b, float c) { float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
+// Columns of tensor memory: three S / P of 128, O'
+constexpr uint32_t COL_S = 0, COL_O = 384;
 
 template <int HD, bool TMA, bool CAP>
 __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map, uint32_t run) {
     using F = AttnTc<HD>;
+    constexpr int LOADERS = TMA ? 1 : TC_LOADERS;        // arrivals of fetched keys or values
     extern __shared__ uint8_t raw[];
     __shared__ AttnRow s_row[TC_ROWS];
     __shared__ float s_unit[TC_ROWS];
     __shared__ uint32_t s_tmem, s_dead;
     __shared__ Found s_found;
-    __shared__ int64_t s_where[2][TMA ? 1 : TC_CB];
-    __shared__ End<TC_ROWS, 2> s_end;
-    // chunk c, stage c & 1: its keys are there / its scores are (and its keys read); its values / its weights / its output (and its values read)
-    __shared__ __align__(8) uint64_t b_k[2], b_s[2], b_v[2], b_p[2], b_o[2];
+    __shared__ int64_t s_where[4][TMA ? 1 : TC_CB];
+    __shared__ End<TC_ROWS, 1> s_end;
+    __shared__ float s_ref[4][TC_ROWS], s_m[2][TC_ROWS], s_l[2][TC_ROWS];     // what a chunk's weights are relative to; maxima and sums of the two
+    // Of chunk c, stage c & 1: its keys are there, are read; its values are there and the output before it is taken, its values are
+    // read.  Slot c % 3: its scores are there; its weights are, are read.  c & 3: s_ref is there (its next user is four chunks on, when
+    // the output of the next one is asked for).  Its output is there.
+    __shared__ __align__(8) uint64_t b_k[2], b_kr[2], b_v[2], b_vr[2], b_s[3], b_p[3], b_pr[3], b_ref[4], b_o;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t kvh = blockIdx.y, split = blockIdx.x % a.splits, t = gridDim.x / a.splits - 1 - blockIdx.x / a.splits;   // late rows see more: first
+    const AttnShare part = share_of(a);
+    const uint32_t kvh = part.kvh;
     AttnTile x;
-    if (!find_tile<TC_ROWS, TC_CB>(a, t, kvh, x, s_row, s_found)) return;
+    if (!find_tile<TC_ROWS, TC_CB>(a, part.tile, kvh, x, s_row, s_found)) return;
     uint32_t sharers, c0, c1;
-    if (!share_out(a, x, split, sharers, c0, c1)) return;
+    if (!share_out(a, x, part, sharers, c0, c1)) return;
     const int n = (int)(c1 - c0);
     uint8_t* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const uint32_t sm_s = smem_u32(sm);
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], TMA ? 1 : TC_LOADERS); mbar_init(&b_s[i], 1); mbar_init(&b_v[i], TMA ? 1 : TC_LOADERS); mbar_init(&b_p[i], 128); mbar_init(&b_o[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], LOADERS); mbar_init(&b_kr[i], 1); mbar_init(&b_v[i], LOADERS + 256); mbar_init(&b_vr[i], 1); }
+        for (int i = 0; i < 3; ++i) { mbar_init(&b_s[i], 1); mbar_init(&b_p[i], 128); mbar_init(&b_pr[i], 1); }
+        mbar_init(&b_o, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&b_ref[i], 128);
         s_dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 11) {
+    if (warp == TC_ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // queries: two fp16 terms of the row times a power of two (with the sign of the scale), four rows of a warp under way at once
-    constexpr int W = TC_THREADS / 32, VPL = HD / 32, R4 = 4;
-#pragma unroll 1
-    for (int r1 = warp; r1 < TC_ROWS; r1 += R4 * W) {
-        float v[R4][VPL];
+    atc_fence_before();
+    __syncthreads();
+    atc_fence_after();
+    const uint32_t tmem = s_tmem;
+    // queries, by all but the warps that fetch (they begin) and issue: two fp16 terms of the row times a power of two (with the
+    // sign of the scale), a warp's rows all under way at once
+    constexpr int W = TC_FETCH, VPL = HD / 32, R = TC_ROWS / W;
+    if (warp < TC_FETCH) {
+        float v[R][VPL];
 #pragma unroll
-        for (int j = 0; j < R4; ++j) {
-            const int r = r1 + j * W;
-            const bool on = r < TC_ROWS && s_row[r].pos >= 0;
+        for (int j = 0; j < R; ++j) {
+            const int r = warp + j * W;
+            const bool on = s_row[r].pos >= 0;
             const float* src = a.act + (on ? s_row[r].q : 0);
 #pragma unroll
             for (int i = 0; i < VPL; ++i) v[j][i] = on ? src[lane + 32 * i] : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < R4; ++j) {
-            const int r = r1 + j * W;
-            if (r >= TC_ROWS) break;
+        for (int j = 0; j < R; ++j) {
+            const int r = warp + j * W;
             float most = 0.f, up, down;
 #pragma unroll
             for (int i = 0; i < VPL; ++i) most = fmaxf(most, fabsf(v[j][i]));
@@ -147,20 +180,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             }
         }
     }
-    atc_proxy_fence();
-    atc_fence_before();
-    __syncthreads();
-    atc_fence_after();
-    const uint32_t tmem = s_tmem;
+    if (warp >= TC_FETCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else atc_proxy_fence();
+    if (warp < TC_FETCH || warp >= TC_ISSUE) asm volatile("bar.sync 2, %0;" :: "n"(TC_THREADS - TC_LOADERS) : "memory");
     bool dead = false;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {        // bounded: what comes later then does not wait any more
-        if (!dead && !mbar_wait(bar, parity)) { dead = true; s_dead = 1; atomicOr(a.err, DEVERR_WAIT); }
+    auto wait1 = [&](uint64_t* bar, uint32_t parity) {       // bounded: what comes later then does not wait any more
+        if (dead) return;
+#pragma unroll 1
+        for (int spin = 0; !atc_try(bar, parity); ++spin)
+            if (spin == 1 << 20) { dead = true; s_dead = 1; atomicOr(a.err, DEVERR_WAIT); return; }
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {        // a warp (one lane that asks for the others takes 2900 cycles a chunk to 3160)
+        wait1(bar, parity);
+        __syncwarp();
     };
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (TMA && warp == 8) {
-            // ---- keys and values, a run of positions of one page to a copy; the swizzle is the copy's ----
+    if (warp >= TC_FETCH) {
+        if (TMA && warp < TC_ISSUE) {
+            // ---- keys (one warp) and values (another: neither waits for the other's stage), a run of positions of one page to a copy;
+            // the swizzle is the copy's ----
+            const bool keys = warp == TC_FETCH;
             const uint32_t runs = TC_CB / run;
             const int32_t outside = (int32_t)(a.pool_rows);      // no row of the pool: a copy from there brings zeros
             auto locate = [&](int c) -> int32_t {
@@ -168,157 +207,194 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
                 const int32_t p = chunk_at<TC_CB>(x, c0 + c) + lane * (int32_t)run;
                 if (p > x.hi || (p + (int32_t)run <= x.from && (uint32_t)p >= a.n_sink)) return outside;
                 const int32_t page = x.pages[(uint32_t)p / a.geo.page];
-                return page < 0 ? outside : (int32_t)(kv_index(a.geo, (uint32_t)page, a.layer, 0, kvh, (uint32_t)p % a.geo.page) / HD);
+                return page < 0 ? outside : (int32_t)(kv_index(a.geo, (uint32_t)page, a.layer, keys ? 0 : 1, kvh, (uint32_t)p % a.geo.page) / HD);
             };
-            const int32_t v_row = (int32_t)(a.geo.n_kv * a.geo.page);
-            int32_t row = locate(0);
-            auto fetch = [&](int c, int32_t y, uint32_t base, uint64_t* free, uint64_t* full) {
-                if (c >= 2) wait(free, (uint32_t)((c >> 1) - 1) & 1u);
-                if (lane == 0) mbar_expect_tx(full, F::PLANE);
+            const uint32_t to = sm_s + (keys ? F::K : F::V) + lane * run * 128;
+            uint64_t *const full = keys ? b_k : b_v, *const free = keys ? b_kr : b_vr;
+            int32_t y = locate(0);
+            for (int c = 0; c < n; ++c) {
+                const int32_t next = locate(c + 1);
+                uint64_t* const bar = full + (c & 1);
+                if (c >= 2) wait(free + (c & 1), (uint32_t)((c >> 1) - 1) & 1u);
+                if (lane == 0) mbar_expect_tx(bar, F::PLANE);
                 __syncwarp();
                 if ((uint32_t)lane < runs)
 #pragma unroll
                     for (int d0 = 0; d0 < HD; d0 += 64)
                         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                                     :: "r"(sm_s + base + (uint32_t)(c & 1) * F::PLANE + (d0 >> 6) * TC_BLOCK + lane * run * 128), "l"(&map), "r"(d0), "r"(y), "r"(smem_u32(full)) : "memory");
-            };
-            for (int c = 0; c < n; ++c) {
-                const int32_t next = locate(c + 1);
-                fetch(c, row, F::K, &b_s[c & 1], &b_k[c & 1]);
-                fetch(c, row == outside ? outside : row + v_row, F::V, &b_o[c & 1], &b_v[c & 1]);
-                row = next;
+                                     :: "r"(to + (uint32_t)(c & 1) * F::PLANE + (d0 >> 6) * TC_BLOCK), "l"(&map), "r"(d0), "r"(y), "r"(smem_u32(bar)) : "memory");
+                y = next;
             }
             // nothing is under way when the CTA ends, also where a wait ran out
-            for (int c = max(n - 2, 0); c < n; ++c) { mbar_wait(&b_k[c & 1], (uint32_t)(c >> 1) & 1u); mbar_wait(&b_v[c & 1], (uint32_t)(c >> 1) & 1u); }
-        } else if (!TMA && warp < 11) {
+            for (int c = max(n - 2, 0); c < n; ++c) mbar_wait(full + (c & 1), (uint32_t)(c >> 1) & 1u);
+        } else if (!TMA && warp < TC_ISSUE) {
             // ---- keys and values, 16 bytes at a time ----
-            const int me = tid - 256;
+            const int me = (warp - TC_FETCH) * 32 + lane;
             const __half* const pool = reinterpret_cast<const __half*>(a.pool);
             const size_t v_off = (size_t)a.geo.n_kv * a.geo.page * HD;
             constexpr int WPR = HD / 8;                      // 16-byte words of a row
             uint64_t* owed = nullptr;                        // whose copies are under way and not yet announced
             auto announce = [&]() { atc_proxy_fence(); atc_arrive(owed); owed = nullptr; };
             auto fetch = [&](int c, uint32_t base, size_t off, uint64_t* free, uint64_t* full) {
-                if (c >= 2 && !atc_try(free, (uint32_t)((c >> 1) - 1) & 1u)) {
+                if (c >= 2 && !__all_sync(0xffffffffu, atc_try(free, (uint32_t)((c >> 1) - 1) & 1u))) {
                     if (owed) { at_wait<0>(); announce(); }
                     wait(free, (uint32_t)((c >> 1) - 1) & 1u);
                 }
 #pragma unroll 4
                 for (int w = me; w < TC_CB * WPR; w += TC_LOADERS) {
                     const int r = w / WPR, ch = w % WPR;
-                    const int64_t at = s_where[c & 1][r];
+                    const int64_t at = s_where[c & 3][r];
                     at_cp16(sm_s + base + (uint32_t)(c & 1) * F::PLANE + tc_at(r, ch * 8), pool + (at < 0 ? 0 : (size_t)at + off) + ch * 8, at >= 0);
                 }
                 at_commit();
                 if (owed) { at_wait<1>(); announce(); }
                 owed = full;
             };
-            for (int c = 0; c < n; ++c) {
+            auto locate = [&](int c) {                       // (behind the barrier before it everybody is done with chunk c - 4)
+                if (c >= n) return;
                 const int32_t p0 = chunk_at<TC_CB>(x, c0 + c);
-                for (int r = me; r < TC_CB; r += TC_LOADERS) s_where[c & 1][r] = tile_position(a, x, kvh, p0 + r);
+                for (int r = me; r < TC_CB; r += TC_LOADERS) s_where[c & 3][r] = tile_position(a, x, kvh, p0 + r);
+            };
+            // in the order of their use: keys a chunk ahead of values
+            for (int c = 0; c < n + 1; ++c) {
+                locate(c);
                 asm volatile("bar.sync 1, %0;" :: "n"(TC_LOADERS) : "memory");
-                fetch(c, F::K, 0, &b_s[c & 1], &b_k[c & 1]);
-                fetch(c, F::V, v_off, &b_o[c & 1], &b_v[c & 1]);
+                if (c < n) fetch(c, F::K, 0, &b_kr[c & 1], &b_k[c & 1]);
+                if (c >= 1) fetch(c - 1, F::V, v_off, &b_vr[(c - 1) & 1], &b_v[(c - 1) & 1]);
             }
             at_wait<0>();
             if (owed) announce();
-        } else if (warp == 11 && lane == 0) {
-            // ---- products: S of chunk c + 1 goes ahead of O' of chunk c ----
-            auto scores = [&](int c) {
-                const int b = c & 1;
-                wait(&b_k[b], (uint32_t)(c >> 1) & 1u);
+        } else if (warp == TC_ISSUE && lane == 0) {
+            // ---- scores.  A thread that issues is held up until all but a few of its products are done, and a wait beside busy shared
+            // memory takes 350 cycles: with one thread for both kinds the tensor core stood still for 1500 of 4200 cycles a chunk ----
+            const uint32_t q_hi = tc_desc_lo(sm_s + F::Q, 16), q_lo = tc_desc_lo(sm_s + F::Q + F::PLANE, 16), k_0 = tc_desc_lo(sm_s + F::K, 16);
+            for (int c = 0; c < n && !dead; ++c) {
+                wait1(&b_k[c & 1], (uint32_t)(c >> 1) & 1u);
+                if (c >= 3) wait1(&b_pr[c % 3], (uint32_t)(c / 3 - 1) & 1u);         // the weights that lie there are read
                 atc_fence_after();
-                if (dead) return;
-#pragma unroll
+                if (dead) break;
+                const uint32_t d = tmem + COL_S + c % 3 * 128, kd = k_0 + (c & 1) * (F::PLANE >> 4);
+#pragma unroll 1
                 for (int pass = 0; pass < 2; ++pass)         // the low terms first: they are added while the sum is small
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
-                        const uint32_t off = (uint32_t)(k >> 2) * TC_BLOCK + (k & 3) * 32;
-                        atc_mma_ss(tmem + COL_S + b * 128, tc_desc(sm_s + F::Q + (1 - pass) * F::PLANE + off, 16, 1024),
-                                   tc_desc(sm_s + F::K + b * F::PLANE + off, 16, 1024), ATC_IDESC<128, false>, pass + k > 0);
+                        const uint32_t off = ((k >> 2) * TC_BLOCK + (k & 3) * 32) >> 4;
+                        atc_mma_ss(d, tc_desc((pass ? q_hi : q_lo) + off), tc_desc(kd + off), ATC_IDESC<128, false>, pass + k > 0);
                     }
-                atc_commit(&b_s[b]);
-            };
-            auto output = [&](int c) {
-                const int b = c & 1;
-                wait(&b_v[b], (uint32_t)(c >> 1) & 1u);
-                wait(&b_p[b], (uint32_t)(c >> 1) & 1u);
+                atc_commit(&b_s[c % 3]);
+                atc_commit(&b_kr[c & 1]);
+            }
+        } else if (warp == TC_ISSUE + 1 && lane == 0) {
+            // ---- outputs ----
+            const uint32_t v_0 = tc_desc_lo(sm_s + F::V, TC_BLOCK);
+            for (int c = 0; c < n; ++c) {
+                wait1(&b_v[c & 1], (uint32_t)(c >> 1) & 1u);
+                wait1(&b_p[c % 3], (uint32_t)(c / 3) & 1u);
                 atc_fence_after();
-                if (dead) return;
-#pragma unroll
+                if (dead) break;
+                const uint32_t d = tmem + COL_O, pd = tmem + COL_S + c % 3 * 128, vd = v_0 + (c & 1) * (F::PLANE >> 4);
+#pragma unroll 1
                 for (int pass = 0; pass < 2; ++pass)
 #pragma unroll
                     for (int k = 0; k < TC_CB / 16; ++k)
-                        atc_mma_ts(tmem + COL_O + b * HD, tmem + COL_S + b * 128 + k * 16 + (1 - pass) * 8,
-                                   tc_desc(sm_s + F::V + b * F::PLANE + k * 2048, TC_BLOCK, 1024), ATC_IDESC<HD, true>, pass + k > 0);
-                atc_commit(&b_o[b]);
-            };
-            scores(0);
-            for (int c = 0; c < n; ++c) {
-                if (c + 1 < n) scores(c + 1);
-                output(c);
+                        atc_mma_ts(d, pd + k * 16 + (1 - pass) * 8, tc_desc(vd + k * (2048 >> 4)), ATC_IDESC<HD, true>, pass + k > 0);
+                atc_commit(&b_o);
+                atc_commit(&b_pr[c % 3]);
+                atc_commit(&b_vr[c & 1]);
             }
         }
         __syncwarp();
         __syncthreads();
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        // ---- weights and sums: a row to a thread, every other chunk ----
-        const int w = warp >> 2, r = tid & 127;
-        const uint32_t col = tmem + ((uint32_t)(warp & 3) << 21), s_col = col + COL_S + w * 128, o_col = col + COL_O + w * HD;
-        const int32_t pos = s_row[r].pos;
-        // scores to powers of two: times k2, or cap2 tanh of them times k2
-        const float unit = s_unit[r] * fabsf(a.scale), k2 = CAP ? unit * __frcp_rn(a.cap) : unit * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f;
-        float o[HD], m = -INFINITY, l = 0.f, alpha = 0.f;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+    } else if (warp >= TC_OUT) {
+        // ---- outputs: half a row to a thread ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        constexpr int HALF = HD / 2;
+        const int r = tid & 127, half = (warp - TC_OUT) >> 2;
+        const uint32_t o_col = tmem + ((uint32_t)(warp & 3) << 21) + COL_O + half * HALF;
+        float2 o[HALF / 2];
+        float top = -INFINITY;
+        atc_arrive(&b_v[0]);                                 // no output before the first one
 #pragma unroll
-        for (int d = 0; d < HD; ++d) o[d] = 0.f;
-        auto collect = [&](int c, float factor) {            // O' of chunk c to the outputs before it, times `factor`
-            wait(&b_o[w], (uint32_t)(c >> 1) & 1u);
+        for (int d = 0; d < HALF / 2; ++d) o[d] = make_float2(0.f, 0.f);
+        for (int c = 0; c < n; ++c) {
+            wait(&b_ref[c & 3], (uint32_t)(c >> 2) & 1u);
+            const float ref = s_ref[c & 3][r], now = fmaxf(top, ref), to = now == -INFINITY ? 0.f : now;
+            const float alpha = at_exp2(top - to), beta = at_exp2(ref - to);
+            top = now;
+            wait(&b_o, (uint32_t)c & 1u);
             atc_fence_after();
             float v[2][16];
             atc_ld16(o_col, v[0]);
 #pragma unroll
-            for (int d0 = 0; d0 < HD; d0 += 16) {
+            for (int d0 = 0; d0 < HALF; d0 += 16) {
                 float (&u)[16] = v[d0 / 16 & 1];
                 atc_ld_wait(u);
-                if (d0 + 16 < HD) atc_ld16(o_col + d0 + 16, v[(d0 / 16 + 1) & 1]);
+                if (d0 + 16 < HALF) atc_ld16(o_col + d0 + 16, v[(d0 / 16 + 1) & 1]);
+                else { atc_fence_before(); atc_arrive(&b_v[(c + 1) & 1]); }
 #pragma unroll
-                for (int d = 0; d < 16; ++d) o[d0 + d] = fmaf(o[d0 + d], factor, u[d]);
+                for (int d = 0; d < 16; d += 2) {
+                    float2& y = o[(d0 + d) / 2];
+                    y = at_fma2(y, make_float2(alpha, alpha), at_mul2(make_float2(u[d], u[d + 1]), make_float2(beta, beta)));
+                }
             }
-        };
+        }
+        __syncthreads();                                     // all products are done, shared memory is free
+        float l = 0.f;
+        for (int w = 0; w < 2; ++w) l += s_l[w][r] * End<TC_ROWS, 1>::weight<true>(s_m[w][r], top);
+        if (half == 0) { s_end.m[0][r] = top; s_end.l[0][r] = l; }
+        float* to = reinterpret_cast<float*>(sm) + r * (HD + 4) + half * HALF;
+#pragma unroll
+        for (int d = 0; d < HALF; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d / 2].x, o[d / 2].y, o[d / 2 + 1].x, o[d / 2 + 1].y);      // all times 256, like the sums
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        // ---- weights and sums: a row to a thread, every other chunk ----
+        const int w = warp >> 2, r = tid & 127;
+        const uint32_t col = tmem + ((uint32_t)(warp & 3) << 21) + COL_S;
+        const int32_t pos = s_row[r].pos;
+        // scores to powers of two: times k2, or cap2 tanh of them times k2
+        const float unit = s_unit[r] * fabsf(a.scale), k2 = CAP ? unit * __frcp_rn(a.cap) : unit * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f;
+        float m = -INFINITY, l = 0.f;
         for (int c = w; c < n; c += 2) {
             const int32_t p0 = chunk_at<TC_CB>(x, c0 + c);
             const bool all = tile_sees(a, x, p0, TC_CB);
             // position p0 + j is seen for j <= j1 and (j > j0 or j < js)
             const int32_t j1 = pos - p0, j0 = a.window ? j1 - (int32_t)a.window : -1, js = (int32_t)min(a.n_sink, 0x40000000u) - p0;
             auto seen = [&](int j) { return j <= j1 && (j > j0 || j < js); };
-            wait(&b_s[w], (uint32_t)(c >> 1) & 1u);
+            const uint32_t s_col = col + c % 3 * 128;
+            wait(&b_s[c % 3], (uint32_t)(c / 3) & 1u);
             atc_fence_after();
             // Two turns over the scores, 16 columns at a time with the next ones under way: the maximum, the weights.  Loops of two
             // steps, one for chunks that every row sees whole, one for the others: unrolled with every choice inside, the turns took
             // 5500 cycles, most of them fetching instructions.
-            constexpr int STEP = 16;
-            float v[2][STEP], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
-            atc_ld16(s_col, v[0]);
+            constexpr int STEP = 8;
+            float v[2][STEP], mx[2] = {-INFINITY, -INFINITY};
+            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            atc_ld8(s_col, v[0]);
             auto maximum = [&](auto whole) {
 #pragma unroll 1
                 for (int i = 0; i < TC_CB; i += 2 * STEP)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         atc_ld_wait(v[h]);
-                        atc_ld16(s_col + (i + (h + 1) * STEP) % TC_CB, v[1 - h]);
+                        atc_ld8(s_col + (i + (h + 1) * STEP) % TC_CB, v[1 - h]);
 #pragma unroll
-                        for (int d = 0; d < STEP; ++d) mx[d & 3] = fmaxf(mx[d & 3], decltype(whole)::value || seen(i + h * STEP + d) ? v[h][d] : -INFINITY);
+                        for (int d = 0; d < STEP; d += 2) {
+                            auto score = [&](int e) { return decltype(whole)::value || seen(i + h * STEP + e) ? v[h][e] : -INFINITY; };
+                            mx[d >> 1 & 1] = atc_max3(mx[d >> 1 & 1], score(d), score(d + 1));
+                        }
                     }
             };
             if (all) maximum(std::true_type{});
             else maximum(std::false_type{});
-            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            float top = fmaxf(mx[0], mx[1]);
             top = CAP ? cap2 * at_tanh(top * k2) : top * k2;
             const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, shift = 8.f - ref;      // times 256: the low terms stay clear of the subnormals
-            const float before = alpha;
-            alpha = atc_exp2(m - ref);
+            const float alpha = at_exp2(m - ref);
             m = mn;
+            s_ref[c & 3][r] = mn;
+            atc_arrive(&b_ref[c & 3]);
             auto turn = [&](auto whole) {
 #pragma unroll 1
                 for (int i = 0; i < TC_CB; i += 2 * STEP)
@@ -326,62 +402,62 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
                     for (int h = 0; h < 2; ++h) {
                         float (&u)[STEP] = v[h];
                         atc_ld_wait(u);
-                        if (i + h * STEP + STEP < TC_CB) atc_ld16(s_col + i + (h + 1) * STEP, v[1 - h]);
+                        if (i + h * STEP + STEP < TC_CB) atc_ld8(s_col + i + (h + 1) * STEP, v[1 - h]);
                         uint32_t hi[STEP / 2], lo[STEP / 2];
 #pragma unroll
-                        for (int d = 0; d < STEP; ++d) {
-                            u[d] = atc_exp2(CAP ? fmaf(at_tanh(u[d] * k2), cap2, shift) : fmaf(u[d], k2, shift));
-                            if (!decltype(whole)::value && !seen(i + h * STEP + d)) u[d] = 0.f;
+                        for (int d = 0; d < STEP; d += 2) {
+                            float2 y = make_float2(u[d], u[d + 1]);
+                            if (CAP) y = at_fma2(make_float2(at_tanh(y.x * k2), at_tanh(y.y * k2)), make_float2(cap2, cap2), make_float2(shift, shift));
+                            else y = at_fma2(y, make_float2(k2, k2), make_float2(shift, shift));
+                            y.x = at_exp2(y.x); y.y = at_exp2(y.y);
+                            if (!decltype(whole)::value) { if (!seen(i + h * STEP + d)) y.x = 0.f; if (!seen(i + h * STEP + d + 1)) y.y = 0.f; }
+                            sum[d >> 1 & 1] = at_add2(sum[d >> 1 & 1], y);
+                            at_split_h(y.x, y.y, hi[d / 2], lo[d / 2]);
                         }
-#pragma unroll
-                        for (int d = 0; d < STEP / 2; ++d) { sum[d & 3] += u[2 * d] + u[2 * d + 1]; at_split_h(u[2 * d], u[2 * d + 1], hi[d], lo[d]); }
-                        atc_st8(s_col + i + h * STEP, hi);
-                        atc_st8(s_col + i + h * STEP + 8, lo);
+                        const uint32_t at = (uint32_t)((i + h * STEP) & ~15) + ((i + h * STEP) & 15) / 2;
+                        atc_st4(s_col + at, hi);
+                        atc_st4(s_col + at + 8, lo);
                     }
             };
             if (all) turn(std::true_type{});
             else turn(std::false_type{});
-            l = fmaf(l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-            if (c >= 2) collect(c - 2, before);              // its products ran meanwhile; O' is free for this chunk's
+            const float2 both = at_add2(sum[0], sum[1]);
+            l = fmaf(l, alpha, both.x + both.y);
             atc_st_wait();
             atc_fence_before();
-            atc_arrive(&b_p[w]);
+            atc_arrive(&b_p[c % 3]);
         }
-        if (n > w) collect((n - 1 - w) / 2 * 2 + w, alpha);
-        s_end.m[w][r] = m; s_end.l[w][r] = l * (1.f / 256.f);
+        s_m[w][r] = m; s_l[w][r] = l;
         atc_fence_before();
-        __syncthreads();                                     // all products are done, shared memory is free
-        const float f = s_end.factor<true>(w, r) * (1.f / 256.f);
-        float* to = reinterpret_cast<float*>(sm) + (w * TC_ROWS + r) * (HD + 4);
-#pragma unroll
-        for (int d = 0; d < HD; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d] * f, o[d + 1] * f, o[d + 2] * f, o[d + 3] * f);
+        __syncthreads();
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     }
     atc_fence_after();
     __syncthreads();
-    if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
+    if (warp == TC_ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     if (s_dead) return;
-    settle<__half, HD, TC_ROWS, 2, TC_THREADS, true, false>(a, x, s_row, t, kvh, split, sharers, reinterpret_cast<float*>(sm), s_end);
+    settle<__half, HD, TC_ROWS, 1, TC_THREADS, true, false>(a, x, s_row, part, sharers, reinterpret_cast<float*>(sm), s_end);
 }
 
 template <int HD, bool TMA, bool CAP>
-static int launch_tc(const AttnArgs& a, const KvCache& kv, uint32_t tiles) {
+static int launch_tc(const AttnArgs& a, const KvCache& kv) {
     static bool set = false;
     if (!set) {
         if (cudaFuncSetAttribute((const void*)k_attn_tc<HD, TMA, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttnTc<HD>::SMEM) != cudaSuccess)
             return fail(ADAMAH_ERR_BACKEND, "attn_kv: cannot raise the shared-memory limit");
         set = true;
     }
-    k_attn_tc<HD, TMA, CAP><<<dim3(tiles * a.splits, a.geo.n_kv), TC_THREADS, AttnTc<HD>::SMEM, g.stream>>>(a, kv.map, kv.run);
+    k_attn_tc<HD, TMA, CAP><<<attn_grid(a), TC_THREADS, AttnTc<HD>::SMEM, g.stream>>>(a, kv.map, kv.run);
     count_launch();
     return check_launch("map_attn_kv");
 }
 template <int HD, bool TMA>
-static int launch_cap(const AttnArgs& a, const KvCache& kv, uint32_t tiles) {
-    return a.cap > 0.f ? launch_tc<HD, TMA, true>(a, kv, tiles) : launch_tc<HD, TMA, false>(a, kv, tiles);
+static int launch_cap(const AttnArgs& a, const KvCache& kv) {
+    return a.cap > 0.f ? launch_tc<HD, TMA, true>(a, kv) : launch_tc<HD, TMA, false>(a, kv);
 }
-int launch_attn_tc(const AttnArgs& a, const KvCache& kv, uint32_t tiles) {
-    if (kv.run) return a.geo.hd == 64 ? launch_cap<64, true>(a, kv, tiles) : launch_cap<128, true>(a, kv, tiles);
-    return a.geo.hd == 64 ? launch_cap<64, false>(a, kv, tiles) : launch_cap<128, false>(a, kv, tiles);
+int launch_attn_tc(const AttnArgs& a, const KvCache& kv) {
+    if (kv.run) return a.geo.hd == 64 ? launch_cap<64, true>(a, kv) : launch_cap<128, true>(a, kv);
+    return a.geo.hd == 64 ? launch_cap<64, false>(a, kv) : launch_cap<128, false>(a, kv);
 }
 
 }  // namespace ab

@@ -377,6 +377,67 @@ def test_attention(gpu, heads, kv_heads, dim, dtype, kind):
     c.close()
 
 
+WIDE = [
+    # what is chosen by how much there is: type, dims, query heads of a key head, page, new rows and earlier positions, window, sinks, cap
+    ("f16", 64, 2, 16, [140, 1, 60], [900, 400, 1000], 0, 0, 0.0),
+    ("f16", 64, 3, 12, [140, 1, 60], [900, 400, 1000], 0, 0, 50.0),
+    ("f16", 128, 2, 64, [400, 33], [300, 900], 250, 5, 50.0),
+    ("f16", 128, 1, 12, [400, 33], [300, 900], 250, 5, 0.0),
+    ("f16", 128, 4, 8, [129, 128, 127], [1100, 0, 555], 0, 0, 0.0),
+    ("f16", 256, 2, 64, [150], [1000], 0, 0, 50.0),
+    ("f16", 256, 8, 64, [250], [1300], 0, 0, 0.0),
+    ("f32", 128, 2, 64, [150, 20], [1000, 3], 0, 0, 0.0),
+    ("f32", 128, 8, 16, [250], [1300], 0, 0, 50.0),
+    ("f32", 256, 8, 64, [250], [1300], 0, 0, 0.0),
+    ("f32", 256, 2, 5, [150], [1000], 0, 0, 0.0),
+    ("f32", 64, 2, 16, [140, 1, 60], [900, 400, 1000], 64, 70, 0.0),
+    ("f16", 32, 2, 16, [140, 1, 60], [900, 400, 1000], 100, 0, 0.0),
+]
+
+
+@pytest.mark.parametrize("dtype,dim,group,page,new,ctx,window,n_sink,cap", WIDE)
+def test_attention_of_much(gpu, dtype, dim, group, page, new, ctx, window, n_sink, cap):
+    rng = np.random.default_rng(dim + page)
+    lens = [n + p for n, p in zip(new, ctx)]
+    heads = 8 * group
+    c = Cache(gpu, 1, 8, dim, page, len(new), max(-(-x // page) for x in lens), sum(-(-x // page) for x in lens) + 1, dtype)
+    c.fill(rng, lens, poison=True)
+    starts = np.cumsum([0] + new)
+    q = (rng.standard_normal((starts[-1], heads, dim)) * 2.5).astype(np.float32)
+    got = attention(gpu, c, list(range(len(new))), starts, int(starts[-1]), heads, q, 0, window, n_sink, cap=cap)
+    assert np.isfinite(got).all()
+    want, rows, most = [], [], 0.0
+    for s, n in enumerate(new):
+        for i in sorted({*range(0, n, 11), n - 1}):
+            o, m = ko.attend(q[starts[s] + i], c.held[s][:, 0, 0], c.held[s][:, 0, 1], ctx[s] + i, window, n_sink, dim ** -0.5, cap)
+            want.append(o), rows.append(starts[s] + i)
+            most = max(most, m)
+    near(got[rows], np.stack(want), most)
+    assert gpu.device_error() == 0
+    c.close()
+
+
+@pytest.mark.parametrize("dtype,dim,page", [("f16", 64, 12), ("f16", 128, 16), ("f32", 128, 16), ("f16", 256, 64)])
+def test_attention_of_much_with_infinite_and_nan_values(gpu, dtype, dim, page):
+    rng = np.random.default_rng(dim)
+    n, new, window = 1200, 150, 900
+    c = Cache(gpu, 1, 8, dim, page, 1, n // page + 1, n // page + 1, dtype)
+    c.fill(rng, [n], poison=True)
+    pool, table = c.pool(), gpu.kv_table(c.id)[0]
+    for p, which, value in [(n - 1, 0, np.nan), (n - 1, 1, np.inf), (n - 4, 1, -np.inf), (60, 0, np.inf), (61, 1, np.nan), (n - new - window, 1, np.inf)]:
+        c.held[0][p, 0, which, 0, 3] = value
+        pool[int(table[p // page]), 0, which, 0, p % page, 3] = float(value)
+    q = rng.standard_normal((new, 16, dim)).astype(np.float32)
+    got = attention(gpu, c, [0], [0, new], new, 16, q, layer=0, window=window)
+    rows = [*range(0, new - 8, 13), *range(new - 8, new)]
+    with np.errstate(all="ignore"):
+        want = np.stack([ko.attend(q[r], c.held[0][:, 0, 0], c.held[0][:, 0, 1], n - new + r, window, 0, dim ** -0.5, 0.0)[0] for r in rows])
+    got, fine = got[rows], np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)].astype(np.float32))
+    assert (np.abs(got[fine] - want[fine]) <= 1e-4).all()
+    c.close()
+
+
 def test_attention_rows_anywhere(gpu):
     """Unaligned and permuted rows, results in the queries' place, rows outside every entry, padding entries."""
     rng = np.random.default_rng(9)
