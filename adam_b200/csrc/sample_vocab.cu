@@ -26,11 +26,23 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t SV_SUBS = 256;                    // stretches of a CTA's share, a sum for each
 constexpr uint32_t SV_RESIDENT = 36864;              // logits that a CTA keeps in shared memory at most
-constexpr uint32_t SV_TABLE = 1024;
+constexpr uint32_t SV_TABLE = 1024, SV_GATHER = 8192;
 constexpr uint32_t SV_NEAR_BINS = 256;
 enum SvMode { SV_COUNT, SV_NEAR, SV_EXACT };
+__device__ __forceinline__ float2 sv_fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 sv_add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
 constexpr int SV_T = 1024, SV_W = SV_T / 32;
-constexpr uint32_t SV_BINS = 2048, SV_FEW = 2048;    // bins; candidates that one CTA sorts
+constexpr uint32_t SV_BINS = 2048, SV_FEW = 2048, SV_SHORT = 512;      // bins; candidates that one CTA sorts, that it sorts twice rather than all others sum up
 
 struct SampleArgs {
     float* map; uint64_t n_el;
@@ -58,30 +70,84 @@ __device__ __forceinline__ uint64_t warp_scan_u64(uint64_t v) {      // inclusiv
     return v;
 }
 
-// Weights as integers.  (max - x) / (T ln 2) = y is formed in two 32-bit words; 2^-y = 2^-k 2^(-i/1024) (1 - s) with the table's
-// entry i, an integer k and s = 1 - 2^-r, |r| <= 2^-11, whose series needs two terms (the third is 7e-12).  A weight is known to
-// 5e-10 of itself, so what is drawn changes with probability 1e-7 or so.  What the last unit cuts off is half a unit in the
-// mean: the weights are odd numbers of half units.
+// 2^30 2^(-i/1024), by the series of the exponential
+struct SvTable {
+    uint32_t w[SV_TABLE];
+    constexpr SvTable() : w{} {
+        for (uint32_t i = 0; i < SV_TABLE; ++i) {
+            const double z = -(double)i / SV_TABLE * 0.69314718055994530942;
+            double sum = 1.0, term = 1.0;
+            for (int n = 1; n < 20; ++n) { term *= z / n; sum += term; }
+            w[i] = (uint32_t)(sum * 1073741824.0 + 0.5);
+        }
+    }
+};
+__device__ const SvTable sv_table{};
+
+// Weights as integers.  With C = 1024 / (T ln 2), 1024 log2 of a weight is max C - x C.  max C is once split into the nearest integer
+// and a rest; of -x C the nearest integer n comes from one fma whose sum has no room for a fraction, the rest from a second
+// one, exact but for its own rounding (2^-26), and the low word of C.  2^-(k + i/1024 + r/1024) = 2^-k 2^(-i/1024) (1 - q): the
+// table's entry i, an integer k, and |r| <= 1.3, for which three terms of the series leave 1e-14.  A weight is known to 5e-10 of
+// itself (the table's and the product's 30 bits), so what is drawn changes with probability 1e-7 or so.  What the last unit cuts
+// off is half a unit in the mean: the weights are odd numbers of half units.  (Fewer instructions than with max - x in two words,
+// and those on floats two at a time: 64 rows of 262144, all weights once: 63 -> 55 us.)
 struct SvWeights {
-    const uint32_t* table;                            // 2^30 2^(-i/1024)
-    float mx, c_hi, c_lo; int shift;
-    __device__ __noinline__ uint64_t special(float x) const {        // no finite difference, or nothing left of the weight
+    const uint32_t* table;
+    float mx, low, c_hi, c_lo, rest; int32_t whole; int shift; double c;      // logits up to `low` are no matter of the two fmas
+    __device__ __forceinline__ void init(const uint32_t* t, float most, float temperature, int units) {
+        table = t; mx = most; shift = units;
+        c = 1.4426950408889634074 / (double)temperature;
+        const double C = c * SV_TABLE, all = (double)mx * C, limit = 4095.0;
+        c_hi = (float)C; c_lo = (float)(C - (double)c_hi);
+        const bool fine = fabs(all) < limit * SV_TABLE && c < 1e30;
+        whole = fine ? __double2int_rn(all) : 0;
+        rest = fine ? (float)(all - (double)whole) : 0.f;
+        const double per = 0.69314718055994530942 * (double)temperature;       // a halving of the weight
+        low = fine ? (float)fmax((double)mx - ((double)shift - 0.5) * per, -limit * per) : INFINITY;
+    }
+    __device__ __noinline__ static uint64_t special(float x, float mx, double c, int shift) {       // far below, not a number, or a product that is too large
         if (x == mx) return 1ull << shift | 1u;
-        if (!(mx - x > 3.402823466e+38f) || mx > 3.402823466e+38f) return 0;
-        const double w = exp2(-(((double)mx - (double)x) * ((double)c_hi + (double)c_lo)));       // the difference of two logits overflows
-        return (uint64_t)(w * (double)(1ull << shift)) | (w > 0.0 ? 1u : 0u);
+        if (!(x < mx) || mx > 3.402823466e+38f) return 0;
+        const double y = ((double)mx - (double)x) * c;
+        return y < (double)shift ? (uint64_t)(exp2(-y) * (double)(1ull << shift)) | 1u : 0;
+    }
+    __device__ __forceinline__ uint64_t units(float t, float cut) const {
+        constexpr float MAGIC = 12582912.f;
+        const int32_t ti = __float_as_int(t) - __float_as_int(MAGIC) + whole;
+        const int w = (int)table[ti & (SV_TABLE - 1)];
+        return ((uint64_t)(uint32_t)(w + __mulhi(w, __float_as_int(cut) - __float_as_int(MAGIC))) << 33) >> (63 - shift + (ti >> 10)) | 1u;
+    }
+    __device__ __forceinline__ void pair(float2 x, uint64_t& a, uint64_t& b) const {         // both above `low`
+        constexpr float MAGIC = 12582912.f, K = 0.69314718055994530942f / SV_TABLE;     // 1.5 x 2^23: sums with it are integers
+        const float2 minus = make_float2(-x.x, -x.y), ch = make_float2(c_hi, c_hi);
+        const float2 t = sv_fma2(minus, ch, make_float2(MAGIC, MAGIC)), n = sv_add2(t, make_float2(-MAGIC, -MAGIC));
+        const float2 r = sv_add2(sv_fma2(minus, ch, make_float2(-n.x, -n.y)), sv_fma2(minus, make_float2(c_lo, c_lo), make_float2(rest, rest)));
+        // q 2^32 = -(z - z^2 / 2 + z^3 / 6) 2^32,  z = K r
+        constexpr float TWO32 = 4294967296.f;
+        float2 q = sv_fma2(r, make_float2(-K * K * K / 6.f * TWO32, -K * K * K / 6.f * TWO32), make_float2(K * K / 2.f * TWO32, K * K / 2.f * TWO32));
+        q = sv_fma2(r, q, make_float2(-K * TWO32, -K * TWO32));
+        q = sv_fma2(r, q, make_float2(MAGIC, MAGIC));
+        a = units(t.x, q.x);
+        b = units(t.y, q.y);
     }
     __device__ __forceinline__ uint64_t operator()(float x) const {
-        constexpr float MAGIC = 12582912.f;            // 1.5 x 2^23: the low bits of a sum with it are the nearest integer
-        const float d = mx - x, b = d - mx, d_lo = (mx - (d - b)) + (-x - b);
-        const float y = d * c_hi;
-        if (!(y < (float)shift)) return special(x);    // below a unit, or not a number
-        const float t = fmaf(y, (float)SV_TABLE, MAGIC);
-        const float r = fmaf(t - MAGIC, -1.f / SV_TABLE, y) + (fmaf(d, c_hi, -y) + fmaf(d, c_lo, d_lo * c_hi));
-        const float z = r * 0.69314718055994530942f, q = fmaf(z * z, -0.5f, z);
-        const uint32_t ti = __float_as_uint(t) & 0x3fffffu;
-        const int w = (int)table[ti % SV_TABLE], cut = __float_as_int(fmaf(q, 4294967296.f, MAGIC)) - __float_as_int(MAGIC);
-        return ((uint64_t)(uint32_t)(w - __mulhi(w, cut)) << 33) >> (63 - shift + ti / SV_TABLE) | 1u;
+        if (!(x > low)) return special(x, mx, c, shift);
+        uint64_t a, b;
+        pair(make_float2(x, x), a, b);
+        return a;
+    }
+    __device__ __forceinline__ void four(const float4& x, uint64_t (&w)[4]) const {
+        if (x.x > low && x.y > low && x.z > low && x.w > low) {
+            pair(make_float2(x.x, x.y), w[0], w[1]);
+            pair(make_float2(x.z, x.w), w[2], w[3]);
+        } else {
+            const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t y = (*this)(j < 2 ? (j ? v[1] : v[0]) : (j > 2 ? v[3] : v[2]));
+                if (j == 0) w[0] = y; else if (j == 1) w[1] = y; else if (j == 2) w[2] = y; else w[3] = y;
+            }
+        }
     }
 };
 
@@ -92,11 +158,11 @@ struct SvShared {
     uint32_t table[SV_TABLE];
     uint64_t seg_v, pass_v, all_v, above_v;           // weight of that share; of what is kept, of all, of the bins ahead of the window
     uint64_t kmin, kmax, least;                       // of the crossing bin; the last that is kept
-    uint32_t n_list, first, found; float max;
+    uint32_t n_list, first, found, n_gather; float max;
     uint64_t sub_v[SV_SUBS], wv[SV_W];
     float wmax[SV_W];
-    uint64_t hit_above, hit_v, hit_count; uint32_t hit_bin, hit_n;
-    uint64_t peer_v[16];
+    uint64_t hit_above, hit_v; uint32_t hit_bin, hit_n, hit_upto;         // hit_upto: how many logits up to the end of the bin
+    uint64_t peer_v[16]; uint32_t seg_n, peer_n[16];
 };
 
 // The first m of the list into falling order by the whole CTA; zeros go last.  Up to 128 by counting the larger ones; beyond
@@ -158,16 +224,25 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     const bool lead = rank == 0 && tid == 0;
     if (ol + a.V > a.n_el || ou >= a.n_el || od >= a.n_el) { if (lead) atomicOr(a.err, DEVERR_OOB_MAP); return; }
     const float u = a.map[ou];
+    for (uint32_t i = tid; i < SV_TABLE; i += SV_T) s.table[i] = sv_table.w[i];
     const uint32_t base = rank * a.chunk, n = base < a.V ? min(a.chunk, a.V - base) : 0u;
     const float* src = a.map + ol + base;
     const bool aligned = ((ol + base) & 3) == 0;
     const float* const at = RES ? sx : src;
     // f(logit, its place in the CTA's share) for each, in no order.  A NaN fails every comparison below, like what is not kept.
+    // After a cut that leaves few of a streamed row, only those that may still be kept.
+    bool gathered = false;
+    float* const gx = sx;
+    uint32_t* const gi = reinterpret_cast<uint32_t*>(sx + SV_GATHER);
     auto each = [&](auto f) {
+        if (!RES && gathered) {
+            for (uint32_t i = tid; i < s.n_gather; i += SV_T) f(gx[i], gi[i]);
+            return;
+        }
         if (RES || aligned) {
             const float4* v4 = reinterpret_cast<const float4*>(at);
             const uint32_t n4 = n / 4;
-#pragma unroll 4
+#pragma unroll 2                                     // (by fours the code that a short row fetches once costs more)
             for (uint32_t i = tid; i < n4; i += SV_T) {
                 const float4 v = v4[i];
                 f(v.x, 4 * i); f(v.y, 4 * i + 1); f(v.z, 4 * i + 2); f(v.w, 4 * i + 3);
@@ -201,7 +276,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     }
     mx = warp_max(mx);
     if (lane == 0) s.wmax[warp] = mx;
-    if (tid == 0) { s.n_list = 0; s.first = 0xffffffffu; }
+    if (tid == 0) { s.n_list = 0; s.first = 0xffffffffu; s.n_gather = 0; }
     __syncthreads();
     if (warp == 0) {
         mx = warp_max(s.wmax[lane]);
@@ -221,17 +296,15 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         if (lead && mx != -INFINITY) a.map[od] = (float)s.first;
         return;
     }
-    for (uint32_t i = tid; i < SV_TABLE; i += SV_T) s.table[i] = __double2uint_rn(exp2(-(double)i / SV_TABLE) * 1073741824.0);
-
-    const double c = 1.4426950408889634074 / (double)rule.temperature;
-    const float c_hi = (float)c;
-    const SvWeights weight{s.table, mx, c_hi, c_hi <= 3.402823466e+38f ? (float)(c - (double)c_hi) : 0.f, a.shift};
+    SvWeights weight;
+    weight.init(s.table, mx, rule.temperature, a.shift);
     const float step = 64.0f / rule.temperature;
-    const uint64_t least = (uint64_t)ceil((double)fminf(fmaxf(rule.min_p, 0.f), 1.f) * (double)(1ull << a.shift));    // of min_p
     auto bin_of = [&](float x) -> uint32_t {
         const float t = (mx - x) * step;
-        return t < (float)(SV_BINS - 1) ? (uint32_t)t : x == mx ? 0u : SV_BINS - 1;
+        return t < (float)(SV_BINS - 1) ? __float_as_uint(__fadd_rd(t, 8388608.f)) & (SV_BINS - 1) : x == mx ? 0u : SV_BINS - 1;      // (a conversion takes 8 cycles)
     };
+
+    const uint64_t least = (uint64_t)ceil((double)fminf(fmaxf(rule.min_p, 0.f), 1.f) * (double)weight(mx));      // of min_p
 
     // ---- the threshold: what is kept are the logits above x_t, and those equal to it up to index i_t ----
     float x_t = -INFINITY;
@@ -259,6 +332,8 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     auto merge = [&](SvMode mode) {
         together();
         uint64_t tv = 0;
+        if (tid == 0) s.seg_n = 0;
+        uint32_t tn = 0;
         for (uint32_t b = tid; b < per; b += SV_T) {
             const uint32_t bin = rank * per + b;
             const bool sums = mode == SV_EXACT || (mode == SV_NEAR && bin < SV_NEAR_BINS);
@@ -272,34 +347,23 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
             if (mode == SV_COUNT) cv = cn;
             else if (!sums) cv = cn * (uint64_t)(exp2f((bin + 0.5f) * (-1.4426950408889634f / 64.f)) * (float)(1ull << a.shift));
             s.all.n[b] = cn; s.all.lo[b] = (uint32_t)cv; s.all.hi[b] = (uint32_t)(cv >> 32);
-            tv += cv;
+            tv += cv; tn += cn;
         }
         tv = warp_sum_u64(tv);
+        tn = __reduce_add_sync(0xffffffffu, tn);
         if (lane == 0) s.wv[warp] = tv;
         __syncthreads();
+        if (mode != SV_COUNT && lane == 0 && tn) atomicAdd(&s.seg_n, tn);
         if (warp == 0) {
             tv = warp_sum_u64(s.wv[lane]);
             if (lane == 0) s.seg_v = tv;
         }
         together();
-        if (tid < C) s.peer_v[tid] = *cl.map_shared_rank(&s.seg_v, tid);
+        if (tid < C) { s.peer_v[tid] = *cl.map_shared_rank(&s.seg_v, tid); s.peer_n[tid] = *cl.map_shared_rank(&s.seg_n, tid); }
         __syncthreads();
     };
     // A value of every CTA, added up
     auto add_up = [&](const uint64_t* mine) { return warp_sum_u64(lane < C ? *cl.map_shared_rank(mine, lane) : 0ull); };
-    // How many logits lie in the bins up to `bin`, from the merged histogram
-    auto upto = [&](uint32_t bin) {
-        uint32_t v = 0;
-        for (uint32_t b = tid; b < per; b += SV_T) v += rank * per + b <= bin ? s.all.n[b] : 0u;
-        v = __reduce_add_sync(0xffffffffu, v);
-        if (tid == 0) s.hit_count = 0;
-        __syncthreads();
-        if (lane == 0) atomicAdd((unsigned long long*)&s.hit_count, (unsigned long long)v);
-        together();
-        const uint64_t all = add_up(&s.hit_count);
-        together();
-        return all;
-    };
     auto total = [&]() { uint64_t v = 0; for (uint32_t k = 0; k < C; ++k) v += s.peer_v[k]; return v; };
     // exclusive sums over the CTA, and the sum of all
     auto scan = [&](uint64_t v, uint64_t& sum) {
@@ -312,19 +376,22 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint64_t before = __shfl_sync(0xffffffffu, ahead, warp ? warp - 1 : 0);
         return incl - v + (warp ? before : 0ull);
     };
-    // The bin in which the running sum reaches `target` (1 .. total), the sum ahead of it, its own and its count: in s.hit_*.
-    auto cross = [&](uint64_t target) {
-        uint64_t above = 0, sum; uint32_t seg = 0;
-        while (seg + 1 < C && above + s.peer_v[seg] < target) above += s.peer_v[seg++];
+    // The bin in which the running sum reaches `target` (1 .. total), the sum ahead of it, its own and its count, and with `counts` how many
+    // logits lie up to its end: in s.hit_*.
+    auto cross = [&](uint64_t target, bool counts) {
+        uint64_t above = 0, sum; uint32_t seg = 0, n_above = 0;
+        while (seg + 1 < C && above + s.peer_v[seg] < target) { n_above += s.peer_n[seg]; above += s.peer_v[seg++]; }
         const SvBins* h = cl.map_shared_rank(&s.all, seg);
         const uint32_t mine = (per + SV_T - 1) / SV_T, b0 = tid * mine;
-        uint64_t v = 0;
-        for (uint32_t b = b0; b < min(b0 + mine, per); ++b) v += (uint64_t)h->lo[b] + ((uint64_t)h->hi[b] << 32);
+        uint64_t v = 0, n_mine = 0;
+        for (uint32_t b = b0; b < min(b0 + mine, per); ++b) { v += (uint64_t)h->lo[b] + ((uint64_t)h->hi[b] << 32); n_mine += h->n[b]; }
         above += scan(v, sum);
+        if (counts) n_above += (uint32_t)scan(n_mine, sum);
         if (above < target && target <= above + v)
             for (uint32_t b = b0; b < min(b0 + mine, per); ++b) {
                 const uint64_t x = (uint64_t)h->lo[b] + ((uint64_t)h->hi[b] << 32);
-                if (target <= above + x) { s.hit_bin = seg * per + b; s.hit_above = above; s.hit_v = x; s.hit_n = h->n[b]; break; }
+                n_above += h->n[b];
+                if (target <= above + x) { s.hit_bin = seg * per + b; s.hit_above = above; s.hit_v = x; s.hit_n = h->n[b]; s.hit_upto = n_above; break; }
                 above += x;
             }
         __syncthreads();
@@ -394,31 +461,43 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         uint32_t* const n_list = cl.map_shared_rank(&s.n_list, 0);
         uint64_t* const list = cl.map_shared_rank(&s.list[0], 0);
         uint64_t t_all = 0, t_above = 0, sum;
-        auto one = [&](float x, uint32_t i) -> uint64_t {
-            if constexpr (!decltype(window)::value) return value(x, i);
-            else {
-                if (!kept(x, i)) return 0;
-                const uint64_t w = weight(x);
-                const uint32_t bin = bin_of(x);
+        // bin_of(x) < b0, <= b1
+        const float t0 = (float)b0, t1 = b1 + 1 < SV_BINS ? (float)(b1 + 1) : INFINITY;
+        auto one = [&](float x, uint32_t i, uint64_t w) -> uint64_t {
+            if (!kept(x, i)) return 0;
+            if constexpr (decltype(window)::value) {
                 t_all += w;
-                if (bin < b0) { t_above += w; return w >= least ? w : 0; }
-                if (bin <= b1) list[atomicAdd(n_list, 1u)] = sv_key(x, base + i);
-                return 0;
+                const float t = (mx - x) * step;
+                if (!(t < t0) && (x != mx || b0 == 0)) {
+                    if (t < t1 || t1 == INFINITY || x == mx) list[atomicAdd(n_list, 1u)] = sv_key(x, base + i);
+                    return 0;
+                }
+                t_above += w;
             }
+            return least <= 1 || w >= least ? w : 0;
         };
-        for (uint32_t b = warp; b < n_sub; b += SV_W) {
+        if (!RES && gathered) {
+            for (uint32_t b = tid; b < n_sub; b += SV_T) s.sub_v[b] = 0;
+            __syncthreads();
+            each([&](float x, uint32_t i) {
+                const uint64_t v = one(x, i, weight(x));
+                if (v) atomicAdd((unsigned long long*)&s.sub_v[i / sub], (unsigned long long)v);
+            });
+        } else for (uint32_t b = warp; b < n_sub; b += SV_W) {
             uint64_t v = 0;
             const uint32_t end = min(n, (b + 1) * sub);
             if (RES || aligned) {
 #pragma unroll 2
                 for (uint32_t i = b * sub + 4 * lane; i + 3 < end; i += 128) {
                     const float4 x = *reinterpret_cast<const float4*>(at + i);
-                    v += one(x.x, i) + one(x.y, i + 1) + one(x.z, i + 2) + one(x.w, i + 3);
+                    uint64_t w[4];
+                    weight.four(x, w);
+                    v += one(x.x, i, w[0]) + one(x.y, i + 1, w[1]) + one(x.z, i + 2, w[2]) + one(x.w, i + 3, w[3]);
                 }
-                if (const uint32_t i = (end & ~3u) + lane; i < end) v += one(at[i], i);
+                if (const uint32_t i = (end & ~3u) + lane; i < end) v += one(at[i], i, weight(at[i]));
             } else {
 #pragma unroll 4
-                for (uint32_t i = b * sub + lane; i < end; i += 32) v += one(at[i], i);
+                for (uint32_t i = b * sub + lane; i < end; i += 32) v += one(at[i], i, weight(at[i]));
             }
             v = warp_sum_u64(v);
             if (lane == 0) s.sub_v[b] = v;
@@ -453,17 +532,21 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     // end.  1: the token is drawn, 0: it is cut, -1: the end lies elsewhere, or too many logits around it.
     auto nucleus = [&]() -> int {
         clear(SV_NEAR);
-        each([&](float x, uint32_t i) { if (kept(x, i)) count(bin_of(x), x, SV_NEAR); });
+        // What all logits below `far` could weigh is less than half the slack of the smallest total: not counted (most of a row that
+        // has some logits far above the others)
+        const float far = mx - (logf((float)a.V) + 7.625f) * rule.temperature;
+        each([&](float x, uint32_t i) { if (x > far && kept(x, i)) count(bin_of(x), x, SV_NEAR); });
         merge(SV_NEAR);
         const uint64_t near = total(), target = share(near), slack = near >> 10;
-        cross(target > slack ? target - slack : 1);
+        cross(target > slack ? target - slack : 1, true);
         uint32_t b0 = s.hit_bin;
-        cross(min(near, target + slack));
+        const uint32_t ahead = s.hit_upto - s.hit_n;
+        cross(min(near, target + slack), true);
         const uint32_t b1 = s.hit_bin;
-        const uint64_t end = upto(b1);
-        bool drawn = whole && end <= SV_FEW;                    // all candidates fit the list
+        const uint32_t end = s.hit_upto;
+        bool drawn = whole && end <= SV_SHORT;                  // all candidates fit a list that is sorted twice
         if (drawn) b0 = 0;
-        else if (end - (b0 ? upto(b0 - 1) : 0) > SV_FEW) return -1;
+        else if (end - ahead > SV_FEW) return -1;
         sweep(std::true_type{}, b0, b1);
         together();
         if (rank == 0) {
@@ -491,7 +574,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         return 0;
     };
     // Cuts what is kept to the run that reaches a target: so many logits (sums false), or so much weight.  True: the token is drawn.
-    auto cut = [&](bool sums) -> bool {
+    auto cut = [&](bool sums) __attribute__((always_inline)) -> bool {         // (a call would put all of these on the stack)
         const SvMode mode = sums ? SV_EXACT : SV_COUNT;
         clear(mode);
         each([&](float x, uint32_t i) { if (kept(x, i)) count(bin_of(x), x, mode); });
@@ -499,11 +582,11 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint64_t all = total();
         if (!sums && all <= rule.top_k) return false;
         const uint64_t target = sums ? share(all) : rule.top_k;
-        cross(target);
+        cross(target, sums);
         const uint32_t bin = s.hit_bin;
         uint64_t rest = target - s.hit_above;
         uint32_t in = s.hit_n;
-        if (whole && (sums ? upto(bin) : s.hit_above + s.hit_v) <= SV_FEW) {          // the first CTA sorts all candidates and does the rest
+        if (whole && (sums ? s.hit_upto : s.hit_above + s.hit_v) <= SV_FEW) {          // the first CTA sorts all candidates and does the rest
             collect([&](float x, uint32_t) { return x > -INFINITY && bin_of(x) <= bin; });
             if (rank == 0) few(sums ? all : 0);
             return true;
@@ -536,13 +619,23 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
             clear(mode);
             each([&](float x, uint32_t i) { if (inside(x, i)) count((uint32_t)((hi - sv_key(x, base + i)) >> sh), x, mode); });
             merge(mode);
-            cross(rest);
+            cross(rest, false);
             in = s.hit_n; rest -= s.hit_above;
             hi -= (uint64_t)s.hit_bin << sh;
             const uint64_t span = (1ull << sh) - 1u;
             lo = hi - lo > span ? hi - span : lo;
         }
-        collect(inside);
+        // (for a streamed row of the bins up to the crossing one all that there is, if it is not too much)
+        if (!RES && !gathered) {
+            collect([&](float x, uint32_t i) {
+                if (x > -INFINITY && bin_of(x) <= bin) {
+                    const uint32_t at = atomicAdd(&s.n_gather, 1u);
+                    if (at < SV_GATHER) { gx[at] = x; gi[at] = i; }
+                }
+                return inside(x, i);
+            });
+            gathered = s.n_gather <= SV_GATHER;          // (behind the wait of all)
+        } else collect(inside);
         if (rank == 0) {
             last_of_list(rest, sums);
             __syncthreads();
@@ -556,7 +649,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     if (rule.top_k > 0 && rule.top_k < a.V && cut(false)) return;
     if (rule.top_p < 1.f) {
         // a weight for every logit twice, here and in the draw, costs less than nucleus() where a CTA has few of them
-        // (a row of 32003 on eight CTAs 17 against 25 us; 64 rows of 262144 on two each 153 against 133)
+        // (a row of 32003 on eight CTAs 17 against 25 us; 64 rows of 262144 on two each 153 against 111)
         const int done = RES ? -1 : nucleus();
         if (done > 0 || (done < 0 && cut(true))) return;
     }
@@ -605,12 +698,12 @@ static int launch_sample(const SampleArgs& a, uint32_t rows, uint32_t C) {
     constexpr size_t fixed = (sizeof(SvShared) + 15) / 16 * 16;
     static bool set = false;
     if (!set) {
-        if (cudaFuncSetAttribute((const void*)k_sample_vocab<RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + (RES ? SV_RESIDENT * 4 : 0))) != cudaSuccess ||
+        if (cudaFuncSetAttribute((const void*)k_sample_vocab<RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + (RES ? SV_RESIDENT * 4 : SV_GATHER * 8))) != cudaSuccess ||
             cudaFuncSetAttribute((const void*)k_sample_vocab<RES>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return fail(ADAMAH_ERR_BACKEND, "sample: cannot set the kernel's limits");
         set = true;
     }
-    launch_k_cluster(k_sample_vocab<RES>, dim3(rows * C), dim3(SV_T), fixed + (RES ? (size_t)a.chunk * 4 : 0), g.stream, false, C, false, a);
+    launch_k_cluster(k_sample_vocab<RES>, dim3(rows * C), dim3(SV_T), fixed + (RES ? (size_t)a.chunk * 4 : SV_GATHER * 8), g.stream, false, C, false, a);
     count_launch();
     return check_launch("map_sample");
 }

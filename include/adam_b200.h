@@ -365,10 +365,10 @@ int map_attn_kv_dev(uint32_t map, uint32_t kv, uint32_t layer, uint32_t q_h, uin
  * The weights are exp((logit - largest) / temperature).  In the order of falling logits, lower index first, the first top_k
  * stay, of those the shortest run whose weights reach top_p of theirs, of those the ones with a weight of min_p or more; the
  * first never goes.  The token is the lowest index whose running sum, in index order, is above u times the sum.  With
- * temperature <= 0 the first is taken.  Weights are rounded to units of 2^-45 of the largest
- * (2^-39 at 2^24 logits), sums of them are exact: what is drawn does not depend on the launch.  Logits of -infinity and NaN are never drawn; a row of
- * nothing else gives -1.  Rules and numbers out of range (NaN, u outside [0, 1)) give -1 and set bit 3 of the device error
- * word. */
+ * temperature <= 0 the first is taken.  A weight is a whole number of units, 2^-45 of the largest at 262144 logits and 2^-39 at
+ * 2^24, right to 5e-10 of itself and half a unit; sums of them are exact, so what is drawn does not depend on the launch.
+ * Logits of -infinity and NaN are never drawn; a row of nothing else gives -1.  Rules and numbers out of range (NaN, u outside
+ * [0, 1)) give -1 and set bit 3 of the device error word. */
 typedef struct adam_b200_sample_rule {
     float    temperature;
     uint32_t top_k;              /* 0: all */

@@ -59,6 +59,21 @@ def test_rules_and_sizes(gpu, rows, vocab):
     check(gpu, logits, RULES, rng.random(rows).astype(np.float32), pad=rows % 3)
 
 
+@pytest.mark.parametrize("kind", ["peaked", "flat", "steps"])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_rows_too_long_to_keep(gpu, kind, pad):
+    """A CTA's share does not fit its shared memory; both cuts one after the other, of little and of much, ties across the cut."""
+    rows, vocab = 12, 700001
+    rng = np.random.default_rng(len(kind) + pad)
+    x = rng.standard_normal((rows, vocab)) * 2.5
+    if kind == "peaked":
+        x += 14.0 * rng.random((rows, vocab)) ** (vocab / 40)
+    logits = (np.round(x * 4) / 4 if kind == "steps" else x).astype(np.float32)
+    rules = [(1.1, 5000, 0.99, 0.01), (1.0, 20000, 0.9, 0.0), (3.0, 200000, 0.95, 0.0), (0.7, 0, 0.9, 0.0), (1.0, 0, 0.9, 0.02), (2.0, 700000, 0.5, 0.0),
+             (0.02, 3000, 0.999, 0.0), (1.0, 300, 0.9, 0.1), (1.0, 0, 0.01, 0.0), (50.0, 0, 0.999, 0.0), (0.9, 2500, 1.0, 0.0), (1.0, 0, 1.0, 0.3)]
+    check(gpu, logits, rules, rng.random(rows).astype(np.float32), pad=pad)
+
+
 @pytest.mark.parametrize("vocab", [5, 3000, 50000, 262144])
 def test_ties(gpu, vocab):
     """Few distinct logits: cuts fall inside groups of equal ones, of which the lowest indices stay."""
