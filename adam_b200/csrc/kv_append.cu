@@ -59,7 +59,7 @@ __device__ __forceinline__ void st_vals(__half* p, bool, const float (&x)[N]) { 
 // A CTA per row at a time; its warps take the row's heads.  Lane l has the dims N l .. of both halves.
 template <typename T, int HD>
 __global__ void __launch_bounds__(AP_T) k_kv_append(const AppendArgs a) {
-    constexpr int HALF = HD / 2, N = HALF >= 32 ? HALF / 32 : 1;
+    constexpr int HALF = HD / 2, N = HALF >= 32 ? HALF / 32 : 1, W = AP_T / 32, U = N == 4 ? 2 : 4;
     __shared__ __align__(16) float s_cos[HALF], s_sin[HALF];
     __shared__ int s_entry;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -85,6 +85,20 @@ __global__ void __launch_bounds__(AP_T) k_kv_append(const AppendArgs a) {
             if (threadIdx.x == 0) atomicOr(a.err, DEVERR_OOB_MAP);
             continue;
         }
+        // U heads of a warp at a time: all their values are asked for before the first is used
+        float x0[U][N], x1[U][N];
+        auto ask = [&](uint32_t h0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t h = h0 + u * W;
+                const bool is_q = h < a.n_head, is_v = h >= a.n_head + n_kv;
+                const uint64_t at = is_q ? oq + (uint64_t)h * HD : (is_v ? ov : ok) + (uint64_t)(h - a.n_head - (is_v ? n_kv : 0)) * HD;
+#pragma unroll
+                for (int j = 0; j < N; ++j) { x0[u][j] = 0.f; x1[u][j] = 0.f; }
+                if (on && h < heads) { ld_vals<N>(a.act + at + i0, at % N == 0, x0[u]); ld_vals<N>(a.act + at + i0 + HALF, at % N == 0, x1[u]); }
+            }
+        };
+        ask(warp);
         if (threadIdx.x < HALF) {
             const double t = (double)pos * turn;
             sincospif(2.0f * (float)(t - rint(t)), &s_sin[threadIdx.x], &s_cos[threadIdx.x]);
@@ -95,39 +109,45 @@ __global__ void __launch_bounds__(AP_T) k_kv_append(const AppendArgs a) {
         for (int j = 0; j < N; ++j) { c[j] = on ? s_cos[i0 + j] : 0.f; s[j] = on ? s_sin[i0 + j] : 0.f; }
         T* const cache = reinterpret_cast<T*>(a.pool) + kv_index(a.geo, (uint32_t)page, a.layer, 0, 0, (uint32_t)pos % a.geo.page);
         const size_t head_step = (size_t)a.geo.page * HD, v_step = head_step * n_kv;
-        for (uint32_t h = warp; h < heads; h += AP_T / 32) {
-            const bool is_q = h < a.n_head, is_v = h >= a.n_head + n_kv;
-            const uint32_t kh = is_v ? h - a.n_head - n_kv : h - a.n_head;
-            const uint64_t at = is_q ? oq + (uint64_t)h * HD : (is_v ? ov : ok) + (uint64_t)kh * HD;
-            const float* src = a.act + at + i0;
-            float x0[N] = {}, x1[N] = {};
-            if (on) { ld_vals<N>(src, at % N == 0, x0); ld_vals<N>(src + HALF, at % N == 0, x1); }
-            if (is_v) {
-                T* dst = cache + v_step + kh * head_step + i0;
-                if (on) { st_vals<N>(dst, true, x0); st_vals<N>(dst + HALF, true, x1); }
-                continue;
-            }
-            if (is_q ? a.l_qw != nullptr : a.l_kw != nullptr) {
-                const uint64_t ow = is_q ? oqw : okw;
-                float w0[N] = {}, w1[N] = {}, ss = 0.f;
-                if (on) { ld_vals<N>(a.wt + ow + i0, ow % N == 0, w0); ld_vals<N>(a.wt + ow + i0 + HALF, ow % N == 0, w1); }
+        float qw0[N] = {}, qw1[N] = {}, kw0[N] = {}, kw1[N] = {};
+        if (on && a.l_qw) { ld_vals<N>(a.wt + oqw + i0, oqw % N == 0, qw0); ld_vals<N>(a.wt + oqw + i0 + HALF, oqw % N == 0, qw1); }
+        if (on && a.l_kw) { ld_vals<N>(a.wt + okw + i0, okw % N == 0, kw0); ld_vals<N>(a.wt + okw + i0 + HALF, okw % N == 0, kw1); }
+        for (uint32_t h0 = warp; h0 < heads; h0 += U * W) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) ss = fmaf(x0[j], x0[j], fmaf(x1[j], x1[j], ss));
-                const float rms = sqrtf(warp_sum(ss) * (1.0f / HD) + a.eps), rcp = __frcp_rn(rms);
+            for (int u = 0; u < U; ++u) {
+                const uint32_t h = h0 + u * W;
+                if (h >= heads) break;
+                const bool is_q = h < a.n_head, is_v = h >= a.n_head + n_kv;
+                const uint32_t kh = is_v ? h - a.n_head - n_kv : h - a.n_head;
+                if (is_v) {
+                    T* dst = cache + v_step + kh * head_step + i0;
+                    if (on) { st_vals<N>(dst, true, x0[u]); st_vals<N>(dst + HALF, true, x1[u]); }
+                    continue;
+                }
+                if (is_q ? a.l_qw != nullptr : a.l_kw != nullptr) {
+                    float ss = 0.f;
 #pragma unroll
-                for (int j = 0; j < N; ++j) { x0[j] = div_by(x0[j], rms, rcp) * w0[j]; x1[j] = div_by(x1[j], rms, rcp) * w1[j]; }
-            }
-            float y0[N], y1[N];
+                    for (int j = 0; j < N; ++j) ss = fmaf(x0[u][j], x0[u][j], fmaf(x1[u][j], x1[u][j], ss));
+                    const float rms = sqrtf(warp_sum(ss) * (1.0f / HD) + a.eps), rcp = __frcp_rn(rms);
 #pragma unroll
-            for (int j = 0; j < N; ++j) { y0[j] = x0[j] * c[j] - x1[j] * s[j]; y1[j] = x0[j] * s[j] + x1[j] * c[j]; }
-            if (!on) continue;
-            if (is_q) {
-                const uint64_t d = od + (uint64_t)h * HD;
-                st_vals<N>(a.act + d + i0, d % N == 0, y0); st_vals<N>(a.act + d + i0 + HALF, d % N == 0, y1);
-            } else {
-                T* dst = cache + kh * head_step + i0;
-                st_vals<N>(dst, true, y0); st_vals<N>(dst + HALF, true, y1);
+                    for (int j = 0; j < N; ++j) {
+                        x0[u][j] = div_by(x0[u][j], rms, rcp) * (is_q ? qw0[j] : kw0[j]);
+                        x1[u][j] = div_by(x1[u][j], rms, rcp) * (is_q ? qw1[j] : kw1[j]);
+                    }
+                }
+                float y0[N], y1[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) { y0[j] = x0[u][j] * c[j] - x1[u][j] * s[j]; y1[j] = x0[u][j] * s[j] + x1[u][j] * c[j]; }
+                if (!on) continue;
+                if (is_q) {
+                    const uint64_t d = od + (uint64_t)h * HD;
+                    st_vals<N>(a.act + d + i0, d % N == 0, y0); st_vals<N>(a.act + d + i0 + HALF, d % N == 0, y1);
+                } else {
+                    T* dst = cache + kh * head_step + i0;
+                    st_vals<N>(dst, true, y0); st_vals<N>(dst + HALF, true, y1);
+                }
             }
+            if (h0 + U * W < heads) ask(h0 + U * W);
         }
     }
 }
