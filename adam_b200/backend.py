@@ -341,6 +341,10 @@ class Adamah:
     def _counts(seqs, n):
         """Sequences and a number for each as uint32 arrays; one number stands for all."""
         seqs = np.ascontiguousarray(seqs, np.uint32).reshape(-1)
+        if type(n) is int and 0 <= n < 1 << 32:
+            full = np.empty(seqs.size, np.uint32)
+            full.fill(n)
+            return seqs, full
         n = np.ascontiguousarray(n, np.uint32).reshape(-1)
         if n.size == 1 and seqs.size != 1:
             n = np.full(seqs.size, n[0], np.uint32)

@@ -79,14 +79,13 @@ static int launch_update(const KvCache& kv, const KvCopy* copies, uint32_t n_cop
     return check_launch("kv_update");
 }
 static int send(const KvCache& kv, const KvUpdate& u) {
-    constexpr uint32_t FEW = 60, MANY = 1000;        // records of a launch: 1 KB and 16 KB of parameters
+    constexpr uint32_t FEW = 60, SOME = 250, MANY = 1000;        // records of a launch: 1, 4 and 16 KB of parameters
     size_t c = 0, r = 0;
     int rc = ADAMAH_OK;
     while (!rc && (c < u.copies.size() || r < u.recs.size())) {
-        const size_t left = u.copies.size() - c + u.recs.size() - r, room = left <= FEW ? FEW : MANY;
+        const size_t left = u.copies.size() - c + u.recs.size() - r, room = left <= FEW ? FEW : left <= SOME ? SOME : MANY;
         const uint32_t nc = (uint32_t)std::min(u.copies.size() - c, room), nr = (uint32_t)std::min(u.recs.size() - r, room - nc);
-        rc = room == FEW ? launch_update<FEW>(kv, u.copies.data() + c, nc, u.recs.data() + r, nr)
-                         : launch_update<MANY>(kv, u.copies.data() + c, nc, u.recs.data() + r, nr);
+        rc = (room == FEW ? launch_update<FEW> : room == SOME ? launch_update<SOME> : launch_update<MANY>)(kv, u.copies.data() + c, nc, u.recs.data() + r, nr);
         c += nc; r += nr;
     }
     end_of_op();
