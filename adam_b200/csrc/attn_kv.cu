@@ -495,7 +495,7 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     // as the GPU holds at once, no more than the workspace has room for: 512 tiles on 148 SMs take 3.5 turns, not 4.
     const uint32_t chunk = rows <= 4 ? attn_thin_chunk(kv->elem, hd) : rows == 16 ? 16 : rows == 128 ? 128 : f16 ? 64 : 32;
     a.least = 128 / chunk;
-    const uint32_t slots = sms * (rows <= 4 ? THIN_CTAS : rows == 16 ? 2 : 1), rest = a.pairs % slots;
+    const uint32_t slots = std::min(sms * (rows <= 4 ? THIN_CTAS : rows == 16 ? 2 : 1), KV_SPLIT_CTAS), rest = a.pairs % slots;
     a.whole = a.pairs; a.splits = 1;
     if (rest) {
         a.splits = std::min({slots / rest, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / rest, parts});

@@ -15,7 +15,7 @@
 // The roles execute different code at once, and what all of them need for a chunk has to stay in an instruction cache that a few
 // SMs refill together: with loops unrolled freely it took 2600 cycles a chunk on some SMs and 4000 on others, with short ones (and
 // two values to an instruction) 2900 everywhere.  Of those the tensor core is busy for about 2700: 16 products of 64 cycles for
-// S, 16 of 107 for P V, whose first operand comes from tensor memory (107 also with half the columns).  2048 tokens behind 14000,
+// S, 16 of about 107 for P V, whose first operand is in the tensor memory that two warpgroups write meanwhile.  2048 tokens behind 14000,
 // 32 heads over 16 of 128: 927 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
 #include "attn_kv.cuh"
 #include "gemv_mma.cuh"
@@ -435,7 +435,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     atc_fence_after();
     __syncthreads();
     if (warp == TC_ISSUE) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
-    if (s_dead) return;
+    if (s_dead) {                                        // what it shares stays as no call has left it
+        if (tid == 0 && sharers > 1) atomicInc(a.tickets + part.slot, sharers - 1);
+        return;
+    }
     settle<__half, HD, TC_ROWS, 1, TC_THREADS, true, false>(a, x, s_row, part, sharers, reinterpret_cast<float*>(sm), s_end);
 }
 

@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         // What all logits below `far` could weigh is less than half the slack of the smallest total: not counted (most of a row that
         // has some logits far above the others)
         const float far = mx - (logf((float)a.V) + 7.625f) * rule.temperature;
-        each([&](float x, uint32_t i) { if (x > far && kept(x, i)) count(bin_of(x), x, SV_NEAR); });
+        each([&](float x, uint32_t i) { if (!(x < far) && kept(x, i)) count(bin_of(x), x, SV_NEAR); });
         merge(SV_NEAR);
         const uint64_t near = total(), target = share(near), slack = near >> 10;
         cross(target > slack ? target - slack : 1, true);

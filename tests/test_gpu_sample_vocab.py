@@ -74,6 +74,30 @@ def test_rows_too_long_to_keep(gpu, kind, pad):
     check(gpu, logits, rules, rng.random(rows).astype(np.float32), pad=pad)
 
 
+def test_special_logits_of_rows_too_long_to_keep(gpu):
+    rng = np.random.default_rng(8)
+    rows, vocab = 12, 700001
+    logits = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+    logits[:, 5] = logits[:, 600000] = np.inf            # infinities share what there is
+    logits[3:6] = np.where(rng.random((3, vocab)) < 0.999, -np.inf, logits[3:6])
+    logits[3:6, 5] = logits[3:6, 600000] = 3.0
+    logits[6:9, 5:600001:7] = np.nan
+    logits[6:9, 5] = logits[6:9, 600000] = 1.0
+    logits[9] = 3.0e38 * np.sign(logits[9])
+    logits[9, ::2] = 0.0
+    logits[10], logits[11] = -np.inf, np.nan
+    u = rng.random(rows).astype(np.float32)
+    got, used = draw(gpu, logits, [(1.0, 0, 0.9, 0.0), (np.inf, 0, 0.9, 0.0), (0.7, 3000, 0.9, 0.01)], u)
+    for r in (0, 1, 2):
+        assert got[r] == (5 if u[r] < 0.5 else 600000), (r, u[r], got[r])
+    for r in range(3, 10):
+        x = logits[r].copy()
+        x[np.isnan(x)] = -np.inf
+        want, margin = ko.sample(x, *used[r], u[r])
+        assert got[r] == want or margin < 2.0 ** -36, (r, used[r], u[r], got[r], want, margin)
+    assert got[10] == got[11] == -1 and gpu.device_error() == 0
+
+
 @pytest.mark.parametrize("vocab", [5, 3000, 50000, 262144])
 def test_ties(gpu, vocab):
     """Few distinct logits: cuts fall inside groups of equal ones, of which the lowest indices stay."""
