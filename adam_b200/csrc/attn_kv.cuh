@@ -35,34 +35,51 @@ struct Found { uint32_t seq, row, n, first, len, warp[32]; };
 template <int ROWS, int CHUNK>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t t, uint32_t kvh, AttnTile& x, AttnRow* rows, Found& f) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    uint32_t before = 0;
-    if (tid == 0) f.seq = KV_NO_SEQ;
-    for (uint32_t e0 = 0; e0 < a.b.n_seqs; e0 += blockDim.x) {
-        const uint32_t e = e0 + tid;
-        uint32_t s0 = 0, s1 = 0, seq = KV_NO_SEQ, len = 0;
+    auto entry = [&](uint32_t e, uint32_t& s0, uint32_t& n, uint32_t& seq, uint32_t& len) {
+        uint32_t s1 = 0;
+        s0 = n = len = 0; seq = KV_NO_SEQ;
         if (e < a.b.n_seqs) { s0 = a.b.start[e]; s1 = a.b.start[e + 1]; seq = a.b.seq[e]; }
         if (seq < a.b.max_seqs) len = (uint32_t)a.b.lens[seq];
         const bool fine = s0 <= s1 && s1 <= a.b.n_rows;
         if (!fine) atomicOr(a.err, DEVERR_OOB_MAP);
-        const uint32_t n = fine ? s1 - s0 : 0u, tiles = (n * a.group + ROWS - 1) / ROWS;
-        uint32_t incl = tiles;
+        else n = s1 - s0;
+        return (n * a.group + ROWS - 1) / ROWS;
+    };
+    auto scan = [&](uint32_t v) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= (uint32_t)o) incl += v; }
+        for (int o = 1; o < 32; o <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, v, o); if (lane >= (uint32_t)o) v += y; }
+        return v;
+    };
+    uint32_t len;
+    if (a.b.n_seqs <= 32) {                              // every warp for itself
+        uint32_t s0, n, seq;
+        const uint32_t tiles = entry(lane, s0, n, seq, len), incl = scan(tiles), at = incl - tiles;
+        const uint32_t hit = __ballot_sync(0xffffffffu, at <= t && t < incl);
+        if (!hit) return false;
+        const int e = __ffs(hit) - 1;
+        x.seq = __shfl_sync(0xffffffffu, seq, e); x.row = __shfl_sync(0xffffffffu, s0, e); x.n = __shfl_sync(0xffffffffu, n, e);
+        x.first = (t - __shfl_sync(0xffffffffu, at, e)) * ROWS; len = __shfl_sync(0xffffffffu, len, e);
+    } else {
+        uint32_t before = 0;
+        if (tid == 0) f.seq = KV_NO_SEQ;
+        for (uint32_t e0 = 0; e0 < a.b.n_seqs; e0 += blockDim.x) {
+            uint32_t s0, n, seq;
+            const uint32_t tiles = entry(e0 + tid, s0, n, seq, len), incl = scan(tiles);
+            __syncthreads();
+            if (lane == 31) f.warp[warp] = incl;
+            __syncthreads();
+            uint32_t at = before + incl - tiles;
+            for (uint32_t w = 0; w < warps; ++w) { if (w < warp) at += f.warp[w]; before += f.warp[w]; }
+            if (at <= t && t < at + tiles) { f.seq = seq; f.row = s0; f.n = n; f.first = (t - at) * ROWS; f.len = len; }
+            if (before > t) break;
+        }
         __syncthreads();
-        if (lane == 31) f.warp[warp] = incl;
-        __syncthreads();
-        uint32_t at = before + incl - tiles;
-        for (uint32_t w = 0; w < warps; ++w) { if (w < warp) at += f.warp[w]; before += f.warp[w]; }
-        if (at <= t && t < at + tiles) { f.seq = seq; f.row = s0; f.n = n; f.first = (t - at) * ROWS; f.len = len; }
-        if (before > t) break;
+        x.seq = f.seq; x.row = f.row; x.n = f.n; x.first = f.first; len = f.len;
     }
-    __syncthreads();
-    x.seq = f.seq;
     if (x.seq == KV_NO_SEQ) return false;
     if (x.seq >= a.b.max_seqs) { if (tid == 0) atomicOr(a.err, DEVERR_OOB_MAP); return false; }
-    x.row = f.row; x.n = f.n; x.first = f.first;
     x.pages = a.b.table + (size_t)x.seq * a.geo.max_pages;
-    const int32_t pos0 = (int32_t)f.len - (int32_t)x.n;
+    const int32_t pos0 = (int32_t)len - (int32_t)x.n;
     const uint32_t last = min(x.first + ROWS, x.n * a.group) - 1;
     x.lo = max(pos0 + (int32_t)(x.first / a.group), 0); x.hi = pos0 + (int32_t)(last / a.group);
     for (uint32_t r = tid; r < ROWS; r += blockDim.x) {
@@ -354,7 +371,8 @@ __device__ __forceinline__ void settle(const AttnArgs& a, const AttnTile& x, con
                 }
             }
         } else { v = value(r, d); z = end.l[0][r]; }
-        v = make_float4(v.x / z, v.y / z, v.z / z, v.w / z);
+        const float rcp = __frcp_rn(z);                  // (four divisions took half of this loop's time)
+        v = make_float4(div_by(v.x, z, rcp), div_by(v.y, z, rcp), div_by(v.z, z, rcp), div_by(v.w, z, rcp));
         const float most = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
         if (rows[r].pos >= 0 && !(most <= FLT_TOP)) atomicOr(&end.bad[r >> 5], 1u << (r & 31));
         if constexpr (KEEP) out[j] = v;
