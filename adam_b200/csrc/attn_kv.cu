@@ -494,11 +494,15 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
     // Splits: what fills the GPU once and again is left whole, and the rest (or all, where it is less) divided among as many CTAs
     // as the GPU holds at once, no more than the workspace has room for: 512 tiles on 148 SMs take 3.5 turns, not 4.
     const uint32_t chunk = rows <= 4 ? attn_thin_chunk(kv->elem, hd) : rows == 16 ? 16 : rows == 128 ? 128 : f16 ? 64 : 32;
-    a.least = 128 / chunk;
+    // Positions of a part: 128, but of a short row's 32 or 64 as long as a cluster of 16 has them all (4 heads of 256 over 1: 130 positions
+    // 12.4 -> 9.6 us, 300 14.5 -> 9.7; 1000 in 32s 12.5, in 64s 10.5; 4000 in 64s 18.6, in 128s 16.6)
+    uint32_t unit = 128;
+    while (rows <= 4 && unit > 32 && reach <= unit / 2 * ATTN_CLUSTER) unit /= 2;
+    a.least = std::max(1u, unit / chunk);
     const uint32_t slots = std::min(sms * (rows <= 4 ? THIN_CTAS : rows == 16 ? 2 : 1), KV_SPLIT_CTAS), rest = a.pairs % slots;
     a.whole = a.pairs; a.splits = 1;
     if (rest) {
-        a.splits = std::min({slots / rest, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / rest, parts});
+        a.splits = std::min({slots / rest, KV_SPLIT_CTAS * KV_SPLIT_ROWS / rows / rest, (reach + unit - 1) / unit});
         // The last CTA adds up 128 rows of each: no more of them than the square root of twice the parts (8 heads over 1, 8 tokens
         // behind 8000: 71 us with 63 splits, 32 with 11)
         if (rows == 128)
