@@ -14,9 +14,9 @@
 //
 // The roles execute different code at once, and what all of them need for a chunk has to stay in an instruction cache that a few
 // SMs refill together: with loops unrolled freely it took 2600 cycles a chunk on some SMs and 4000 on others, with short ones (and
-// two values to an instruction) 2900 everywhere.  Of those the tensor core is busy for about 2700: 16 products of 64 cycles for
-// S, 16 of about 107 for P V, whose first operand is in the tensor memory that two warpgroups write meanwhile.  2048 tokens behind 14000,
-// 32 heads over 16 of 128: 927 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
+// two values to an instruction) 2900 everywhere.  The products need 2048 of those at the tensor core's rate, shared memory 2000 for
+// what it hands to them and takes in, and an output waits for the one before it to be taken.  2048 tokens behind 14000, 32
+// heads over 16 of 128: 927 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
 #include "attn_kv.cuh"
 #include "gemv_mma.cuh"
 
