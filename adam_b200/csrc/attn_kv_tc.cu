@@ -155,11 +155,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
         float v[R][VPL];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            const int r = warp + j * W;
-            const bool on = s_row[r].pos >= 0;
-            const float* src = a.act + (on ? s_row[r].q : 0);
+            const AttnRow& row = s_row[warp + j * W];
+            const float* src = a.act + row.q + lane * VPL;
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) v[j][i] = on ? src[lane + 32 * i] : 0.f;
+            for (int i = 0; i < VPL; ++i) v[j][i] = 0.f;
+            if (row.pos < 0) continue;
+            if (row.q % VPL) {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) v[j][i] = src[i];
+            } else if constexpr (VPL == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src);
+                v[j][0] = y.x; v[j][1] = y.y; v[j][2] = y.z; v[j][3] = y.w;
+            } else {
+                const float2 y = *reinterpret_cast<const float2*>(src);
+                v[j][0] = y.x; v[j][1] = y.y;
+            }
         }
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -170,13 +180,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             row_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))), up, down);
             if (lane == 0) s_unit[r] = down;
             if (a.scale < 0.f) up = -up;
+            uint32_t hi[VPL / 2], lo[VPL / 2];
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const float y = v[j][i] * up;
-                const __half hi = __float2half_rn(y);
-                uint8_t* p = sm + F::Q + tc_at(r, lane + 32 * i);
-                *reinterpret_cast<__half*>(p) = hi;
-                *reinterpret_cast<__half*>(p + F::PLANE) = __float2half_rn(y - __half2float(hi));
+            for (int i = 0; i < VPL; i += 2) at_split_h(v[j][i] * up, v[j][i + 1] * up, hi[i / 2], lo[i / 2]);
+            uint8_t* p = sm + F::Q + tc_at(r, lane * VPL);
+            if constexpr (VPL == 4) {
+                *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(p + F::PLANE) = make_uint2(lo[0], lo[1]);
+            } else {
+                *reinterpret_cast<uint32_t*>(p) = hi[0];
+                *reinterpret_cast<uint32_t*>(p + F::PLANE) = lo[0];
             }
         }
     }
