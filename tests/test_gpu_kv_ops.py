@@ -417,6 +417,35 @@ def test_attention_of_much(gpu, dtype, dim, group, page, new, ctx, window, n_sin
     c.close()
 
 
+@pytest.mark.parametrize("dtype,dim,rows", [("f16", 64, 1), ("f32", 64, 2), ("f16", 128, 7), ("f16", 64, 40), ("f32", 128, 40), ("f16", 256, 3)])
+def test_attention_of_many_sequences(gpu, dtype, dim, rows):
+    """More sequences than a CTA has threads, in any order, some without rows, some that are none."""
+    rng = np.random.default_rng(dim + rows)
+    S = 700
+    new = [(i * 5 + 1) % (rows + 1) if i % 9 else 0 for i in range(S)] if rows > 1 else [1] * S
+    lens = [n + (37 * i) % 190 for i, n in enumerate(new)]
+    c = Cache(gpu, 1, 2, dim, 16, S, 16, sum(-(-x // 16) for x in lens) + 1, dtype)
+    c.fill(rng, lens, poison=True)
+    order = rng.permutation(S).tolist()
+    starts = np.cumsum([0] + [new[s] for s in order])
+    seqs = [A.KV_NO_SEQ if i % 50 == 7 else s for i, s in enumerate(order)]
+    q = rng.standard_normal((starts[-1], 4, dim)).astype(np.float32)
+    got = attention(gpu, c, seqs, starts, int(starts[-1]), 4, q, 0, 100, 3)
+    want, at, most = [], [], 0.0
+    for e, s in enumerate(seqs):
+        n = starts[e + 1] - starts[e]
+        if s == A.KV_NO_SEQ:
+            assert (got[starts[e]:starts[e + 1]] == -7).all()
+            continue
+        for i in sorted({0, n - 1} if n else {}):
+            o, m = ko.attend(q[starts[e] + i], c.held[s][:, 0, 0], c.held[s][:, 0, 1], lens[s] - n + i, 100, 3, dim ** -0.5, 0.0)
+            want.append(o), at.append(starts[e] + i)
+            most = max(most, m)
+    near(got[at], np.stack(want), most)
+    assert gpu.device_error() == 0
+    c.close()
+
+
 @pytest.mark.parametrize("dtype,dim,page", [("f16", 64, 12), ("f16", 128, 16), ("f32", 128, 16), ("f16", 256, 64)])
 def test_attention_of_much_with_infinite_and_nan_values(gpu, dtype, dim, page):
     rng = np.random.default_rng(dim)
