@@ -423,10 +423,11 @@ static int launch_many(const AttnArgs& a) {
 template <typename T, int HD>
 static int launch_rows(const AttnArgs& a, const KvCache& kv, uint32_t rows) {
     if (rows <= 4) return launch_attn_thin(a, sizeof(T), rows);
-    if (rows == 16) return launch_few<T, HD>(a);
-    // 32 and 64: the only choice for heads of 256, and floats of 128
-    if constexpr (HD == 256 || (HD == 128 && sizeof(T) == 4)) return rows == 64 ? launch_many<T, HD, 4, 2>(a) : launch_many<T, HD, 2, 4>(a);
-    else return launch_attn_tc(a, kv);
+    if (rows > 16) {                                     // 32 and 64 for heads of 256 and floats of 128, 128 for fp16 heads of 64 and 128
+        if constexpr (HD == 256 || (HD == 128 && sizeof(T) == 4)) return rows == 64 ? launch_many<T, HD, 4, 2>(a) : launch_many<T, HD, 2, 4>(a);
+        else if constexpr (HD > 32 && sizeof(T) == 2) return launch_attn_tc(a, kv);
+    }
+    return launch_few<T, HD>(a);
 }
 template <typename T>
 static int launch_hd(const AttnArgs& a, const KvCache& kv, uint32_t rows) {
@@ -485,7 +486,7 @@ extern "C" int map_attn_kv_dev(uint32_t map, uint32_t kv_id, uint32_t layer, uin
         // 16 where an entry has no more (wider tiles would be empty: 32 entries of 8 tokens behind 1000: 67 us against 85), where the whole is
         // small, so that more CTAs count for more than less reading (16 tokens behind 2000: 20 us against 22; behind 8000 and 64 tokens: 121
         // against 50), and for short rows, where the wider tiles never won.
-        if (flat <= 16ull * entries || work16 <= 7ull * sms || hd * kv->elem <= 64 || (!f16 && hd == 64)) return 16;
+        if (flat <= 16ull * entries || work16 <= 7ull * sms || hd == 32 || (!f16 && hd == 64)) return 16;
         if (f16 && hd <= 128) return 128;
         // 64 for a large whole (1024 tokens behind 8000, heads of 256, 4 over 1: 333 us against 447; 2048 tokens of a prompt: 156 against 115)
         return work64 > 16ull * sms ? 64 : 32;

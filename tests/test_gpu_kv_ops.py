@@ -392,6 +392,9 @@ WIDE = [
     ("f32", 256, 2, 5, [150], [1000], 0, 0, 0.0),
     ("f32", 64, 2, 16, [140, 1, 60], [900, 400, 1000], 64, 70, 0.0),
     ("f16", 32, 2, 16, [140, 1, 60], [900, 400, 1000], 100, 0, 0.0),
+    ("f16", 32, 2, 16, [340, 1, 60], [900, 400, 1000], 0, 0, 0.0),
+    ("f32", 32, 2, 16, [340, 1, 60], [900, 400, 1000], 0, 0, 50.0),
+    ("f32", 64, 4, 16, [340, 1, 60], [900, 400, 1000], 0, 0, 50.0),
 ]
 
 
