@@ -16,7 +16,7 @@
 // SMs refill together: with loops unrolled freely it took 2600 cycles a chunk on some SMs and 4000 on others, with short ones (and
 // two values to an instruction) 2900 everywhere.  The products need 2048 of those at the tensor core's rate, shared memory 2000 for
 // what it hands to them and takes in, and an output waits for the one before it to be taken.  2048 tokens behind 14000, 32
-// heads over 16 of 128: 927 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
+// heads over 16 of 128: 922 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
 #include "attn_kv.cuh"
 #include "gemv_mma.cuh"
 
@@ -71,8 +71,8 @@ __device__ __forceinline__ bool atc_try(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void atc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void atc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void atc_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// 16 consecutive columns of this thread's lane, valid after atc_ld_wait (through which the values pass, so that nothing is
-// computed from them ahead of it); 8 to them
+// 16 or 8 consecutive columns of this thread's lane, valid after atc_ld_wait (through which the values pass, so that nothing is
+// computed from them ahead of it); 4 to them
 __device__ __forceinline__ void atc_ld16(uint32_t t, float (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
@@ -93,10 +93,6 @@ __device__ __forceinline__ void atc_ld_wait(float (&r)[8]) {
 }
 __device__ __forceinline__ void atc_st4(uint32_t t, const uint32_t (&r)[4]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-}
-__device__ __forceinline__ void atc_st8(uint32_t t, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 :: "r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void atc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -378,7 +374,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             const uint32_t s_col = col + c % 3 * 128;
             wait(&b_s[c % 3], (uint32_t)(c / 3) & 1u);
             atc_fence_after();
-            // Two turns over the scores, 16 columns at a time with the next ones under way: the maximum, the weights.  Loops of two
+            // Two turns over the scores, 8 columns at a time with the next ones under way: the maximum, the weights.  Loops of two
             // steps, one for chunks that every row sees whole, one for the others: unrolled with every choice inside, the turns took
             // 5500 cycles, most of them fetching instructions.
             constexpr int STEP = 8;

@@ -9,8 +9,8 @@
 // lowest indices).  Nothing is sorted: a threshold is found by histograms, the first over equal steps of the logit (steps of
 // 1/64 of the temperature, where logits spread evenly), then over the bits in which the logits of the crossing bin differ.
 //
-// Sums of weights decide about whole numbers, so they are exact: weights are 64-bit exponentials rounded to integers, and
-// integers add up to the same sum in any order (32-bit sums over 262144 tokens draw another token once in some hundred
+// Sums of weights decide about whole numbers, so they are exact: weights are integers of up to 50 bits (SvWeights), which add up
+// to the same sum in any order (32-bit sums over 262144 tokens draw another token once in some hundred
 // rows; atomics on floating point another one from launch to launch).
 //
 // A row is a cluster of CTAs, each with its share of the logits in shared memory: one pass over HBM, what follows reads
