@@ -400,19 +400,22 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint64_t p = (uint64_t)((double)fmaxf(rule.top_p, 0.f) * 18446744073709551616.0), t = __umul64hi(p, all) + (p * all != 0 ? 1u : 0u);
         return t ? t : 1ull;
     };
-    // The logits for which `take` says so into the first CTA's list, sorted (SV_FEW at most).
+    // A logit into the first CTA's list.  Only as many as were counted ever come, and those fit; but a streamed row is read again
+    // for every pass, and no store may depend on its being what it was.
+    auto put = [&](float x, uint32_t i) {
+        if (const uint32_t at = atomicAdd(cl.map_shared_rank(&s.n_list, 0), 1u); at < SV_FEW) *cl.map_shared_rank(&s.list[at], 0) = sv_key(x, base + i);
+    };
+    // The logits for which `take` says so, sorted.
     auto collect = [&](auto take) {
-        uint32_t* const n_list = cl.map_shared_rank(&s.n_list, 0);
-        uint64_t* const list = cl.map_shared_rank(&s.list[0], 0);
-        each([&](float x, uint32_t i) { if (take(x, i)) list[atomicAdd(n_list, 1u)] = sv_key(x, base + i); });
+        each([&](float x, uint32_t i) { if (take(x, i)) put(x, i); });
         together();
-        if (rank == 0) sv_sort(s.list, s.n_list);
+        if (rank == 0) sv_sort(s.list, min(s.n_list, SV_FEW));
     };
     constexpr int PER = SV_FEW / SV_T;                      // candidates of a thread
     // All candidates in the list: cut by the whole rule and drawn from there.  top_p is a share of `all`, or of the first
     // top_k (all = 0).
     auto few = [&](uint64_t all) {
-        const uint32_t m = s.n_list, cand = rule.top_k > 0 ? min(m, rule.top_k) : m;
+        const uint32_t m = min(s.n_list, SV_FEW), cand = rule.top_k > 0 ? min(m, rule.top_k) : m;
         uint64_t w[PER], mine = 0, sum;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -458,8 +461,6 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         return w >= least ? w : 0;
     };
     auto sweep = [&](auto window, uint32_t b0, uint32_t b1) {
-        uint32_t* const n_list = cl.map_shared_rank(&s.n_list, 0);
-        uint64_t* const list = cl.map_shared_rank(&s.list[0], 0);
         uint64_t t_all = 0, t_above = 0, sum;
         // bin_of(x) < b0, <= b1
         const float t0 = (float)b0, t1 = b1 + 1 < SV_BINS ? (float)(b1 + 1) : INFINITY;
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
                 t_all += w;
                 const float t = (mx - x) * step;
                 if (!(t < t0) && (x != mx || b0 == 0)) {
-                    if (t < t1 || t1 == INFINITY || x == mx) list[atomicAdd(n_list, 1u)] = sv_key(x, base + i);
+                    if (t < t1 || t1 == INFINITY || x == mx) put(x, i);
                     return 0;
                 }
                 t_above += w;
@@ -533,9 +534,16 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
     auto nucleus = [&]() -> int {
         clear(SV_NEAR);
         // What all logits below `far` could weigh is less than half the slack of the smallest total: not counted (most of a row that
-        // has some logits far above the others)
-        const float far = mx - (logf((float)a.V) + 7.625f) * rule.temperature;
-        each([&](float x, uint32_t i) { if (!(x < far) && kept(x, i)) count(bin_of(x), x, SV_NEAR); });
+        // has some logits far above the others).  Neither is the rest of the bin that `far` lies in: what is counted are whole bins, so
+        // that the bins b0 .. b1 have as many logits as the counts say when the pass below lists them.
+        float far = mx - (logf((float)a.V) + 7.65f) * rule.temperature;
+        uint32_t bins = max(bin_of(far), 1u);                   // (no other logit as near to the largest as the first bin's: not below 1)
+        if (bins >= SV_BINS - 1) { bins = SV_BINS; far = -INFINITY; }          // differences that are not finite, steps of 0
+        each([&](float x, uint32_t i) {
+            if (x < far || !kept(x, i)) return;                 // below far: in bin `bins` or a later one
+            const uint32_t b = bin_of(x);
+            if (b < bins) count(b, x, SV_NEAR);
+        });
         merge(SV_NEAR);
         const uint64_t near = total(), target = share(near), slack = near >> 10;
         cross(target > slack ? target - slack : 1, true);
@@ -550,9 +558,11 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         sweep(std::true_type{}, b0, b1);
         together();
         if (rank == 0) {
-            sv_sort(s.list, s.n_list);
+            const bool fits = s.n_list <= SV_FEW;
+            __syncthreads();                                    // read by all before it is set back
+            if (fits) sv_sort(s.list, s.n_list);
             const uint64_t all = add_up(&s.all_v), above = add_up(&s.above_v), goal = share(all);
-            const bool found = last_of_list(goal > above ? goal - above : 0, true);
+            const bool found = fits && last_of_list(goal > above ? goal - above : 0, true);
             if (found && drawn) few(all);
             if (tid < C) *cl.map_shared_rank(&s.found, tid) = found;       // to everyone's own: who has drawn leaves
             if (tid == 0 && !found) s.n_list = 0;

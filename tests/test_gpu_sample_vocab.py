@@ -74,6 +74,48 @@ def test_rows_too_long_to_keep(gpu, kind, pad):
     check(gpu, logits, rules, rng.random(rows).astype(np.float32), pad=pad)
 
 
+def plausible(x, temperature, top_k, top_p, u, got):
+    """Can ``got`` be drawn with weights right to 5e-10 of themselves and half a unit of 2^-45?  Sums of equal small weights share
+    their rounding, so the borders of the nucleus and of the draw are known to ``off``, not better."""
+    w = np.exp((x.astype(np.longdouble) - x.max()) / temperature)
+    order = np.argsort(-x, kind="stable")[:top_k or None]
+    c = np.cumsum(w[order])
+    off = 5e-10 * (c[-1] - c[0]) + len(x) * 2.0 ** -46
+    least, most = (min(int(np.searchsorted(c, top_p * c[-1] + d)) + 1, len(c)) for d in (-off, off))
+    kept = np.sort(order[:most])
+    off = 2 * off + c[most - 1] - c[least - 1]
+    cum = np.cumsum(w[kept])
+    at = int(np.searchsorted(kept, got))
+    return at < len(kept) and kept[at] == got and cum[at] - w[got] <= u * cum[-1] + off and cum[at] >= u * cum[-1] - off
+
+
+@pytest.mark.parametrize("rows", [20, 5])                   # streamed; in shared memory
+@pytest.mark.parametrize("top_k,temperature", [(0, 1.0), (3000, 0.5), (200000, 2.0)])
+@pytest.mark.parametrize("depth", [20.10165, 20.125])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_groups_of_equal_logits_far_below_the_largest(gpu, rows, top_k, temperature, depth, pad):
+    """A nucleus that takes nearly all of the weight, and most of the vocabulary ``depth`` temperatures below one logit, where the
+    counts of a row too long to keep end (at half a bin of 1/64 temperature, at a bin's edge): a logit or some on this side of
+    it, many on the other."""
+    vocab = 262144
+    rng = np.random.default_rng(top_k + pad + rows)
+    kinds = []
+    for above, below, spread in [(1, vocab, 0), (1500, vocab, 0), (vocab // 2, vocab, 0), (600, 700, 0), (0, 200000, 0.02)]:
+        x = np.full(vocab, -45.0)
+        x[:below] = -depth - 0.005
+        x[:above] = -depth + 0.005
+        x[:below] += spread * (rng.random(min(below, vocab)) - 0.5)
+        kinds.append(x)
+    logits = np.stack([rng.permutation(kinds[r % len(kinds)]) for r in range(rows)])
+    logits[np.arange(rows), rng.integers(0, vocab, rows)] = 0.0
+    logits = (logits * temperature + 3.0).astype(np.float32)
+    u = (1 - 6e-4 * rng.random(rows)).astype(np.float32)
+    got, used = draw(gpu, logits, [(temperature, top_k, p, 0.0) for p in (0.9995, 0.9999, 1 - 2.0 ** -20)], u, pad=pad)
+    for r in range(rows):
+        assert plausible(logits[r], used[r][0], top_k, used[r][2], float(u[r]), got[r]), (r, used[r], float(u[r]), got[r])
+    assert len(set(got.tolist())) > rows // 3 and gpu.device_error() == 0
+
+
 def test_special_logits_of_rows_too_long_to_keep(gpu):
     rng = np.random.default_rng(8)
     rows, vocab = 12, 700001
