@@ -129,10 +129,12 @@ __global__ void __launch_bounds__(AP_T) k_kv_append(const AppendArgs a) {
 #pragma unroll
                     for (int j = 0; j < N; ++j) ss = fmaf(x0[u][j], x0[u][j], fmaf(x1[u][j], x1[u][j], ss));
                     const float rms = sqrtf(warp_sum(ss) * (1.0f / HD) + a.eps), rcp = __frcp_rn(rms);
+                    // squares overflow long before values do: x / infinity is 0, where div_by, which multiplies by the divisor too, makes a NaN
+                    const float d = rms <= 3.402823466e+38f ? rms : 0.f;
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        x0[u][j] = div_by(x0[u][j], rms, rcp) * (is_q ? qw0[j] : kw0[j]);
-                        x1[u][j] = div_by(x1[u][j], rms, rcp) * (is_q ? qw1[j] : kw1[j]);
+                        x0[u][j] = div_by(x0[u][j], d, rcp) * (is_q ? qw0[j] : kw0[j]);
+                        x1[u][j] = div_by(x1[u][j], d, rcp) * (is_q ? qw1[j] : kw1[j]);
                     }
                 }
                 float y0[N], y1[N];

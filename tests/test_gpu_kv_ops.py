@@ -248,6 +248,54 @@ def test_append_far_positions(gpu):
     c.close()
 
 
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_append_rows_whose_squares_overflow_or_vanish(gpu, dtype, dim):
+    """x / sqrt(mean(x^2) + eps) in 32 bits where the mean is infinite (0, and NaN for an infinite value), or 0 with eps = 0 (nothing
+    finite)."""
+    rng = np.random.default_rng(dim)
+    H, KV, rows = 4, 2, 4
+    c = Cache(gpu, 1, KV, dim, 8, 1, 1, 1, dtype)
+    gpu.kv_extend(c.id, [0], rows)
+    n, m = H * dim, KV * dim
+    x = rng.standard_normal((rows, H + 2 * KV, dim)).astype(np.float32)
+    x[0, :, :] *= np.float32(1e25)
+    x[1, 0] *= np.float32(1e20)                                  # one head of the row; its neighbours are what they were
+    x[1, H] *= np.float32(1e37)
+    x[2, 1, 5], x[2, H + 1, dim - 1] = np.inf, -np.inf
+    x[2, 2, 3], x[2, H, 1] = 3e38, -3e38
+    x[3] *= np.float32(1e-30)
+    x[:, H + KV:] = rng.standard_normal((rows, KV, dim))         # values: not normed
+    w = (1 + 0.1 * rng.standard_normal((2, dim))).astype(np.float32)
+    at = np.cumsum([0, rows * n, rows * m, rows * m, rows * n])
+    gpu.map_create_typed(ACT, A.DTYPE_F32, 1, int(at[-1]) + 2 * dim)
+    gpu.scatter_contiguous(ACT, 0, np.concatenate([x[:, :H].reshape(-1), x[:, H:H + KV].reshape(-1), x[:, H + KV:].reshape(-1)]))
+    gpu.scatter_contiguous(ACT, int(at[-1]), w.reshape(-1))
+    r = np.arange(rows)
+    hs = [up(c, o + r * k) for o, k in zip(at, (n, m, m, n))]
+    ws = up(c, [at[-1]]), up(c, [at[-1] + dim])
+    for eps in (0.0, 1e-6):
+        gpu.map_qk_norm_rope_kv_dev(ACT, ACT, c.id, 0, *hs[:3], *ws, hs[3], *c.batch([0], [0, rows]), 1, rows, H, 1e4, eps)
+        got_q = gpu.gather(ACT, np.arange(at[3], at[4], dtype=np.uint32)).view(np.float32).reshape(rows, H, dim)
+        got = c.read(0)
+        with np.errstate(all="ignore"):
+            for i in range(rows):
+                for heads, out, wt in ((slice(0, H), got_q[i], w[0]), (slice(H, H + KV), got[i, 0, 0].astype(np.float32), w[1])):
+                    v = x[i, heads]
+                    y = v / np.sqrt((v * v).mean(-1, keepdims=True, dtype=np.float32) + np.float32(eps))
+                    assert y.dtype == np.float32
+                    want = ko.rotate_normed(y * wt, None, i, 1e4, 0.0)
+                    fine = np.isfinite(want)
+                    assert np.array_equal(np.isfinite(out), fine), (eps, i)
+                    # as in test_append, and 2^-11 of the value in a 16-bit cache; the plain form's own norm adds dim / 32 + 12 half-steps
+                    pair = np.hypot(want[:, :dim // 2], want[:, dim // 2:])
+                    tol = (2 * (dim / 32 + 12) + 24) * U + (0 if dtype == "f32" or heads.start == 0 else 2.0 ** -11)
+                    assert (np.abs(out - want)[fine] <= (tol * np.concatenate([pair, pair], 1) + 2.0 ** -25)[fine]).all()
+        assert (got_q[0] == 0).all() and (got_q[1, 0] == 0).all() and (got[1, 0, 0, 0] == 0).all()
+        assert np.array_equal(got[:, 0, 1], x[:, H + KV:].astype(c.dtype)) and gpu.device_error() == 0
+    c.close()
+
+
 def test_append_leaves_out_what_it_may_not_write(gpu):
     """Padding entries, unknown sequences, positions that the sequence does not have or shares with another."""
     rng = np.random.default_rng(6)
