@@ -176,13 +176,14 @@ __device__ __forceinline__ void row_scale(float most, float& up, float& down) {
     if (most > 0.f && most < 3.0e38f) ex = max(-120, min(120, 134 - (int)((__float_as_uint(most) >> 23) & 0xFFu)));
     up = __uint_as_float((uint32_t)(127 + ex) << 23); down = __uint_as_float((uint32_t)(127 - ex) << 23);
 }
-// tanh(x): below 1/4 its power series (the first term left out is 9e-9 of the value), else 1 - 2 / (1 + e^2x).
+// tanh(x): below 1/4 its power series (the first term left out is 9e-9 of the value), else 1 - 2 / (1 + e^2x).  NaN for NaN: a row
+// with such a score must not come out finite.
 __device__ __forceinline__ float at_tanh_small(float x) {
     const float y = x * x;
     return fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), x);
 }
 __device__ __forceinline__ float at_tanh(float x) {
-    const float d = 1.f + expf(fminf(2.f * x, 80.f));
+    const float d = 1.f + expf(min_nan(2.f * x, 80.f));
     return fabsf(x) < 0.25f ? at_tanh_small(x) : 1.f - div_by(2.f, d, rcp_newton(d));
 }
 

@@ -223,10 +223,15 @@ __device__ __forceinline__ float rcp_newton(float d) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
     return fmaf(r, fmaf(-d, r, 1.0f), r);
 }
-// The larger value, NaN where either is one (fmaxf drops a NaN).
+// The larger, the smaller value, NaN where either is one (fmaxf and fminf drop a NaN).
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // The warp's largest of values that are not negative, NaN if one of them is: their bits are in their order, NaN last.

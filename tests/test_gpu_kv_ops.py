@@ -565,6 +565,65 @@ def test_attention_infinite_and_nan_values(gpu, dtype, new):
     c.close()
 
 
+# type, dims, query heads of a key head, key heads, page, new rows and all positions: tiles of 2 and 4, of 16, of 32 and 64, of 128 with
+# and without tensor copies
+SPECIAL = [("f16", 64, 2, 1, 16, 1, 300), ("f32", 128, 4, 1, 16, 1, 300), ("f16", 256, 4, 1, 64, 1, 700), ("f32", 32, 3, 2, 16, 6, 300), ("f16", 128, 4, 2, 7, 6, 300),
+           ("f16", 32, 2, 8, 16, 150, 1200), ("f16", 64, 2, 8, 16, 150, 1200), ("f16", 64, 2, 8, 12, 150, 1200), ("f16", 128, 2, 8, 16, 150, 1200),
+           ("f16", 128, 1, 16, 12, 150, 1200), ("f32", 64, 2, 8, 16, 150, 1200), ("f32", 128, 2, 8, 16, 150, 1200), ("f16", 256, 2, 8, 64, 150, 1200),
+           ("f32", 256, 8, 8, 64, 150, 1200)]
+
+
+def special(gpu, rng, dtype, dim, group, kv_heads, page, new, n, window, cap, scale, spoil):
+    """Rows of one sequence against the 64-bit form: not finite where that is not, otherwise as near as scores up to 50 allow (near())."""
+    c = Cache(gpu, 1, kv_heads, dim, page, 1, n // page + 1, n // page + 1, dtype)
+    c.fill(rng, [n], poison=True)
+    q = rng.standard_normal((new, kv_heads * group, dim)).astype(np.float32)
+    pool, table = c.pool(), gpu.kv_table(c.id)[0]
+
+    def put(p, which, head, d, value):
+        c.held[0][p, 0, which, head, d] = value
+        pool[int(table[p // page]), 0, which, head, p % page, d] = float(value)
+
+    spoil(q, put)
+    got = attention(gpu, c, [0], [0, new], new, kv_heads * group, q, layer=0, window=window, cap=cap, scale=scale)
+    with np.errstate(all="ignore"):
+        want = np.stack([ko.attend(q[r], c.held[0][:, 0, 0], c.held[0][:, 0, 1], n - new + r, window, 0, scale, cap)[0] for r in range(min(new, 150))])
+    got, fine = got[:len(want)], np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)].astype(np.float32))
+    assert (np.abs(got[fine] - want[fine]) <= 16 * 8 * U * (1 + 50) * np.maximum(1, np.abs(want[fine]))).all()
+    assert gpu.device_error() == 0
+    c.close()
+    return want
+
+
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("dtype,dim,group,kv_heads,page,new,n", SPECIAL)
+def test_attention_special_queries_and_keys(gpu, dtype, dim, group, kv_heads, page, new, n, cap):
+    """An infinite score is the cap with its sign where there is one, a NaN stays one: an infinite key with products of either sign,
+    a NaN key, infinite and NaN queries, some seen by all rows and some by the last ones only."""
+    def spoil(q, put):
+        q[:, (kv_heads - 1) * group:, 9] = np.abs(q[:, (kv_heads - 1) * group:, 9])
+        q[:, -1, 9] *= -1                                         # the last key head's last query head: scores of -infinity
+        put(n - new, 0, kv_heads - 1, 9, np.inf)
+        if kv_heads > 1:
+            q[new // 2, 0, 3], q[new - 1, 0, dim - 1], q[0, 0, 7] = np.nan, np.inf, -np.inf
+            put(n - new // 3, 0, 0, 5, -np.inf)
+        else:
+            q[0, 0, 3] = np.nan
+        if kv_heads > 2:
+            put(n - new // 3, 0, 1, 5, np.nan)
+
+    want = special(gpu, np.random.default_rng(dim + new), dtype, dim, group, kv_heads, page, new, n, 0, cap, dim ** -0.5, spoil)
+    assert np.isnan(want).any() and np.isfinite(want).any()
+
+
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("dtype,dim,group,kv_heads,page,new,n", SPECIAL + [("f16", 64, 2, 16, 16, 600, 1500), ("f16", 128, 2, 16, 12, 600, 1500)])
+def test_attention_scale_of_zero(gpu, dtype, dim, group, kv_heads, page, new, n, cap):
+    """The mean of what a row sees; rows that see nothing of a chunk of positions among others that do (the first of several, too)."""
+    special(gpu, np.random.default_rng(new + dim), dtype, dim, group, kv_heads, page, new, n, 7 * n // 15, cap, 0.0, lambda q, put: None)
+
+
 def test_attention_leaves_out_what_is_not_there(gpu):
     rng = np.random.default_rng(4)
     c = Cache(gpu, 2, 1, 32, 4, 3, 4, 9, "f32")
