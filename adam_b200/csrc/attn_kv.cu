@@ -10,9 +10,9 @@
 // fp32 with the rescaling that the running maximum needs anyway: the tensor core rounds its sums towards zero, and a sum
 // over 65000 positions that never left it would be 2e-4 off.
 //
-// Positions that no row of the tile sees are zeros in shared memory, whatever the cache holds there.  Where a value that some
-// rows see and others do not is an infinity or a NaN, the others' results are NaN (0 times it); results that are not finite
-// are done again by attend_row, which reads only what the row sees.
+// Values of positions that no row of the tile sees are zeros in shared memory, whatever the cache holds there, and scores of
+// such positions are not looked at.  Where a value that some rows see and others do not is an infinity or a NaN, the others' results
+// are NaN (0 times it); results that are not finite are done again by attend_row, which reads only what the row sees.
 #include "attn_kv.cuh"
 
 #include <algorithm>

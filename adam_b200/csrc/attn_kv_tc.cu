@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     __shared__ float s_ref[4][TC_ROWS], s_m[2][TC_ROWS], s_l[2][TC_ROWS];     // what a chunk's weights are relative to; maxima and sums of the two
     // Of chunk c, stage c & 1: its keys are there, are read; its values are there and the output before it is taken, its values are
     // read.  Slot c % 3: its scores are there; its weights are, are read.  c & 3: s_ref is there (its next user is four chunks on, when
-    // the output of the next one is asked for).  Its output is there.
-    __shared__ __align__(8) uint64_t b_k[2], b_kr[2], b_v[2], b_vr[2], b_s[3], b_p[3], b_pr[3], b_ref[4], b_o;
+    // the output of the next one is asked for).  Its output is there.  Values have come that are not all of them seen.
+    __shared__ __align__(8) uint64_t b_k[2], b_kr[2], b_v[2], b_vr[2], b_s[3], b_p[3], b_pr[3], b_ref[4], b_o, b_end;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const AttnShare part = share_of(a);
     const uint32_t kvh = part.kvh;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], LOADERS); mbar_init(&b_kr[i], 1); mbar_init(&b_v[i], LOADERS + 256); mbar_init(&b_vr[i], 1); }
         for (int i = 0; i < 3; ++i) { mbar_init(&b_s[i], 1); mbar_init(&b_p[i], 128); mbar_init(&b_pr[i], 1); }
-        mbar_init(&b_o, 1);
+        mbar_init(&b_o, 1); mbar_init(&b_end, 1);
         for (int i = 0; i < 4; ++i) mbar_init(&b_ref[i], 128);
         s_dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -220,10 +220,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
             };
             const uint32_t to = sm_s + (keys ? F::K : F::V) + lane * run * 128;
             uint64_t *const full = keys ? b_k : b_v, *const free = keys ? b_kr : b_vr;
+            // A copy brings a run whole where the tile sees any of it.  Values that no row sees become zeros before they are announced: 0
+            // times what another sequence has left there could be a NaN, and a row with a NaN is done again by one warp.
+            uint32_t ends = 0;                               // chunks with such values
             int32_t y = locate(0);
             for (int c = 0; c < n; ++c) {
                 const int32_t next = locate(c + 1);
-                uint64_t* const bar = full + (c & 1);
+                const int32_t p0 = chunk_at<TC_CB>(x, c0 + c);
+                const bool is_end = !keys && (p0 + TC_CB > x.hi + 1 || (p0 < x.from && (uint32_t)p0 + TC_CB > a.n_sink));
+                uint64_t* const bar = is_end ? &b_end : full + (c & 1);
                 if (c >= 2) wait(free + (c & 1), (uint32_t)((c >> 1) - 1) & 1u);
                 if (lane == 0) mbar_expect_tx(bar, F::PLANE);
                 __syncwarp();
@@ -232,9 +237,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_attn_tc(const __grid_constant
                     for (int d0 = 0; d0 < HD; d0 += 64)
                         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                                      :: "r"(to + (uint32_t)(c & 1) * F::PLANE + (d0 >> 6) * TC_BLOCK), "l"(&map), "r"(d0), "r"(y), "r"(smem_u32(bar)) : "memory");
+                if (is_end) {
+                    wait(bar, ends++ & 1u);
+#pragma unroll 1
+                    for (int i = lane; i < TC_CB * 8; i += 32) {         // 16 bytes, wherever in its row the swizzle has them
+                        const int32_t p = p0 + i / 8;
+                        if (p <= x.hi && (p >= x.from || (uint32_t)p < a.n_sink)) continue;
+#pragma unroll
+                        for (int d = 0; d < HD / 64; ++d) *reinterpret_cast<uint4*>(sm + F::V + (c & 1) * F::PLANE + d * TC_BLOCK + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    atc_proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) atc_arrive(full + (c & 1));
+                }
                 y = next;
             }
             // nothing is under way when the CTA ends, also where a wait ran out
+            if (ends) mbar_wait(&b_end, (ends - 1) & 1u);
             for (int c = max(n - 2, 0); c < n; ++c) mbar_wait(full + (c & 1), (uint32_t)(c >> 1) & 1u);
         } else if (!TMA && warp < TC_ISSUE) {
             // ---- keys and values, 16 bytes at a time ----

@@ -624,6 +624,34 @@ def test_attention_scale_of_zero(gpu, dtype, dim, group, kv_heads, page, new, n,
     special(gpu, np.random.default_rng(new + dim), dtype, dim, group, kv_heads, page, new, n, 7 * n // 15, cap, 0.0, lambda q, put: None)
 
 
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("dtype,dim,group,kv_heads,page,new,n", SPECIAL + [("f16", 128, 2, 16, 128, 333, 1111), ("f16", 64, 4, 8, 8, 333, 1111), ("f16", 128, 2, 16, 64, 600, 1501)])
+@pytest.mark.parametrize("window,n_sink", [(0, 0), (300, 0), (300, 5), (130, 200)])
+def test_attention_is_the_same_whatever_lies_where_no_row_sees(gpu, dtype, dim, group, kv_heads, page, new, n, cap, window, n_sink):
+    """The same bits over pages whose other positions are NaN (an earlier holder's, say) and over zeros there: behind the sequence's
+    end, between its first positions and its window."""
+    rng = np.random.default_rng(dim + new)
+    heads, n = kv_heads * group, n - 3
+    c = Cache(gpu, 1, kv_heads, dim, page, 1, n // page + 1, n // page + 1, dtype)
+    c.fill(rng, [n], poison=True)
+    pool, table = c.pool(), gpu.kv_table(c.id)[0]
+    if window:
+        import torch
+        p = np.arange(n_sink, max(n - new + 1 - window, n_sink))
+        pool[torch.from_numpy(table[p // page].astype(np.int64)).cuda(), :, :, :, torch.from_numpy(p % page).cuda()] = float("nan")
+    q = rng.standard_normal((new, heads, dim)).astype(np.float32)
+    runs = []
+    for _ in range(2):
+        runs.append(attention(gpu, c, [0], [0, new], new, heads, q, 0, window, n_sink, cap=cap))
+        pool[pool.isnan()] = 0.0
+    assert np.isfinite(runs[0]).all() and np.array_equal(*runs)
+    rows = [0, new // 2, new - 1]
+    want, most = zip(*(ko.attend(q[r], c.held[0][:, 0, 0], c.held[0][:, 0, 1], n - new + r, window, n_sink, dim ** -0.5, cap) for r in rows))
+    near(runs[0][rows], np.stack(want), max(most))
+    assert gpu.device_error() == 0
+    c.close()
+
+
 def test_attention_leaves_out_what_is_not_there(gpu):
     rng = np.random.default_rng(4)
     c = Cache(gpu, 2, 1, 32, 4, 3, 4, 9, "f32")
