@@ -163,10 +163,18 @@ static int create(const adam_b200_kv_desc& desc, uint32_t id) {
 }
 
 bool capturing();
+// By adam_b200_capture_begin, or by the owner of a stream that the library was lent: the books would change once, the device with
+// every replay.
+static bool recording() {
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    if (capturing()) return true;
+    if (cudaStreamIsCapturing(g.stream, &state) != cudaSuccess) { cudaGetLastError(); return true; }      // the default stream beside another's capture
+    return state != cudaStreamCaptureStatusNone;
+}
 static int page_op(uint32_t id, const char* name, KvCache** kv) {
     *kv = get_kv(id);
     if (!*kv) return ADAMAH_ERR_NOT_FOUND;
-    if (capturing()) return fail(ADAMAH_ERR_INVALID, "%s: pages cannot change hands while a graph is being captured", name);
+    if (recording()) return fail(ADAMAH_ERR_INVALID, "%s: pages cannot change hands while a graph is being captured", name);
     return ADAMAH_OK;
 }
 // One call on the pages: the books first, then what changes on the device.  The host's vectors may run out of memory; no
@@ -189,7 +197,7 @@ using namespace ab;
 extern "C" int adam_b200_kv_create(const adam_b200_kv_desc* desc, uint32_t* id_out) {
     if (!ready()) return ADAMAH_ERR_INVALID;
     if (!desc || !id_out) return fail(ADAMAH_ERR_INVALID, "kv_create: null pointer");
-    if (capturing()) return fail(ADAMAH_ERR_INVALID, "kv_create: a graph is being captured");
+    if (recording()) return fail(ADAMAH_ERR_INVALID, "kv_create: a graph is being captured");
     for (uint32_t id = 0; id < MAX_KV; ++id)
         if (!g_kv[id]) {
             int rc;

@@ -160,6 +160,43 @@ def test_page_refusals(gpu):
     c.close()
 
 
+def test_pages_stay_while_the_owner_of_a_lent_stream_captures(gpu):
+    """Another program's capture of the stream that the library works on: operators are recorded, page calls are refused."""
+    import torch
+    rng = np.random.default_rng(31)
+    heads, KV, D = 4, 2, 64
+    c = Cache(gpu, 1, KV, D, 8, 3, 10, 12, "f16")
+    c.fill(rng, [30, 0, 0])
+    gpu.map_create_typed(ACT, A.DTYPE_F32, 1, 2 * heads * D)
+    q_h, o_h, (seq, start) = up(c, [0]), up(c, [heads * D]), c.batch([0], [0, 1])
+    act = torch.as_tensor(gpu.map_array(ACT), device="cuda")
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    gpu.set_stream(st.cuda_stream)
+    gpu.batch_begin()
+    try:
+        with torch.cuda.graph(graph, stream=st):
+            gpu.map_attn_kv_dev(ACT, c.id, 0, q_h, o_h, seq, start, 1, 1, heads, scale=D ** -0.5)
+            for call in (lambda: gpu.kv_extend(c.id, [0], 1), lambda: gpu.kv_fork(c.id, 0, [1], 30), lambda: gpu.kv_truncate(c.id, [0], 3),
+                         lambda: gpu.kv_compact(c.id), lambda: gpu.kv_create(1, 1, 32, 4, 2, 3), lambda: gpu.kv_destroy(c.id)):
+                with pytest.raises(RuntimeError, match="captured"):
+                    call()
+        assert gpu.kv_lens(c.id).tolist() == [30, 0, 0] and gpu.kv_free_pages(c.id) == 8
+        q = torch.from_numpy(rng.standard_normal(heads * D).astype(np.float32)).cuda()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            act[:heads * D] = q
+            graph.replay()
+            gpu.kv_fork(c.id, 0, [1])                              # and are as ever afterwards
+        torch.cuda.synchronize()
+    finally:
+        gpu.batch_end()
+        gpu.set_stream(0)
+    assert gpu.kv_lens(c.id).tolist() == [30, 30, 0]
+    want, most = ko.attend(q.view(heads, D).cpu().numpy(), c.held[0][:, 0, 0], c.held[0][:, 0, 1], 29, 0, 0, D ** -0.5, 0.0)
+    near(act[heads * D:].view(heads, D).cpu().numpy(), want, most)
+    c.close()
+
+
 # ---- norm + rotation + append ------------------------------------------------------------------------------------------
 
 SHAPES = [(4, 1, 256), (32, 16, 128), (14, 2, 64), (9, 3, 32), (5, 5, 64), (3, 1, 128), (10, 2, 256)]
