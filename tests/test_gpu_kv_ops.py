@@ -333,6 +333,53 @@ def test_append_rows_whose_squares_overflow_or_vanish(gpu, dtype, dim):
     c.close()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_append_captured_while_sequences_grow(gpu, dtype):
+    """Two graphs of one cache, each an append of two rows, replayed in turn at lengths, pages and values of their own time."""
+    rng = np.random.default_rng(17)
+    H, KV, D, page = 4, 2, 64, 5
+    c = Cache(gpu, 2, KV, D, page, 2, 30, 60, dtype)
+    c.fill(rng, [1, 7])
+    n, m = H * D, KV * D
+    at = np.cumsum([0, 4 * n, 4 * m, 4 * m, 4 * n, D, D])            # q, k, v, results of both graphs' rows; weights
+    gpu.map_create_typed(ACT, A.DTYPE_F32, 1, int(at[-1]))
+    w = (1 + 0.1 * rng.standard_normal((2, D))).astype(np.float32)
+    ws = up(c, [at[4]]), up(c, [at[5]])
+    graphs = []
+    for g in range(2):                                            # graph g: the last two positions of sequence g
+        hs = [up(c, o + (2 * g + np.arange(2)) * k) for o, k in zip(at, (n, m, m, n))]
+        batch = c.batch([g], [0, 2])
+        gpu.capture_begin()
+        gpu.map_qk_norm_rope_kv_dev(ACT, ACT, c.id, 1, *hs[:3], *ws, hs[3], *batch, 1, 2, H, 1e4, 1e-6)
+        graphs.append(gpu.capture_end())
+    tol = (D / 32 + 24) * U                                          # as in test_append
+    for step in range(3):
+        for s, grow in enumerate((2 + 11 * step, 2 + 3 * step)):
+            gpu.kv_extend(c.id, [s], grow)
+        held, lens = [c.read(s) for s in range(2)], gpu.kv_lens(c.id)
+        x = (rng.standard_normal(4 * (2 * n + 2 * m)) * 3).astype(np.float32)
+        gpu.scatter_contiguous(ACT, 0, np.concatenate([x, w.reshape(-1)]))
+        for g in graphs:
+            gpu.graph_launch(g)
+        after = gpu.gather(ACT, np.arange(at[4], dtype=np.uint32)).view(np.float32)
+        for s in range(2):
+            got = c.read(s)
+            for i in range(2):
+                r, pos = 2 * s + i, int(lens[s]) - 2 + i
+                q, k, v = (x[at[j] + r * z:at[j] + (r + 1) * z].reshape(-1, D) for j, z in ((0, n), (1, m), (2, m)))
+                for y, out, half in ((ko.rotate_normed(q, w[0], pos, 1e4, 1e-6), after[at[3] + r * n:at[3] + (r + 1) * n].reshape(H, D), 0.0),
+                                     (ko.rotate_normed(k, w[1], pos, 1e4, 1e-6), got[pos, 1, 0], 0.0 if dtype == "f32" else 2.0 ** -11)):
+                    pair = np.hypot(y[:, :D // 2], y[:, D // 2:])
+                    assert (np.abs(out - y) <= tol * np.concatenate([pair, pair], 1) + half * (1 + tol) * np.abs(y) + 2.0 ** -25).all()
+                assert np.array_equal(got[pos, 1, 1], v.astype(c.dtype))
+                held[s][pos, 1] = got[pos, 1]
+            assert np.array_equal(got, held[s])
+    for g in graphs:
+        gpu.graph_destroy(g)
+    assert gpu.device_error() == 0
+    c.close()
+
+
 def test_append_leaves_out_what_it_may_not_write(gpu):
     """Padding entries, unknown sequences, positions that the sequence does not have or shares with another."""
     rng = np.random.default_rng(6)
