@@ -845,6 +845,55 @@ def test_attention_on_a_lent_stream(gpu):
     c.close()
 
 
+@pytest.mark.parametrize("page", [64, 60])
+def test_pages_behind_4_billion_elements(gpu, page):
+    """All operators on pages whose elements have numbers of more than 32 bits: append, attention in tiles of 2, 16 and 128, copies."""
+    import torch
+    rng = np.random.default_rng(page)
+    KV, D, heads, n = 8, 128, 16, 1203
+    low = -(-(1 << 32) // (2 * 2 * KV * page * D))                  # pages of 2^32 elements and more
+    need = -(-n // page)
+    c = Cache(gpu, 2, KV, D, page, 3, low, low + need + 2, "f16")
+    gpu.kv_extend(c.id, [0], low * page)
+    gpu.kv_extend(c.id, [1], n)
+    table, pool = gpu.kv_table(c.id)[1], c.pool()
+    assert int(table[:need].min()) * pool[0].numel() >= 1 << 32
+    x = rng.standard_normal((n,) + c.shape).astype(np.float16)
+    p = np.arange(n)
+
+    def rows(seq):
+        t = gpu.kv_table(c.id)[seq]
+        return (torch.from_numpy(t[p // page].astype(np.int64)).cuda(), slice(None), slice(None), slice(None), torch.from_numpy(p % page).cuda())
+
+    pool[rows(1)] = torch.from_numpy(x).cuda()
+    c.held = [None, x, None]
+    before, after, (oq, ok, ov, od), (qw, kw), starts = append(gpu, c, rng, [1], [3], heads, 1)
+    got = pool[rows(1)].cpu().numpy()
+    for i in range(3):
+        k, v = (before[o[i]:o[i] + KV * D].reshape(KV, D) for o in (ok, ov))
+        y = ko.rotate_normed(k, kw, n - 3 + i, 1e6, 1e-6)
+        assert np.abs(got[n - 3 + i, 1, 0] - y).max() <= 2.0 ** -10 * np.abs(y).max() and np.array_equal(got[n - 3 + i, 1, 1], v.astype(np.float16))
+        x[n - 3 + i, 1] = got[n - 3 + i, 1]
+    assert np.array_equal(got, x)
+    for new in (1, 6, 400):
+        q = rng.standard_normal((new, heads, D)).astype(np.float32)
+        out = attention(gpu, c, [1], [0, new], new, heads, q)
+        at = sorted({0, new // 2, new - 1})
+        want, most = zip(*(ko.attend(q[r], x[:, 1, 0], x[:, 1, 1], n - new + r, 0, 0, D ** -0.5, 0.0) for r in at))
+        near(out[at], np.stack(want), max(most))
+    gpu.kv_fork(c.id, 1, [2])
+    gpu.kv_extend(c.id, [2], 1)                                      # a copy of the last page's positions
+    assert np.array_equal(pool[rows(2)].cpu().numpy(), x)
+    gpu.kv_truncate(c.id, [0])
+    assert gpu.kv_compact(c.id) == need + 1 and gpu.kv_table(c.id).max() == need
+    gpu.sync()
+    for s in (1, 2):
+        assert np.array_equal(pool[rows(s)].cpu().numpy(), x)
+    assert gpu.device_error() == 0
+    del pool
+    c.close()
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
