@@ -400,22 +400,23 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
         const uint64_t p = (uint64_t)((double)fmaxf(rule.top_p, 0.f) * 18446744073709551616.0), t = __umul64hi(p, all) + (p * all != 0 ? 1u : 0u);
         return t ? t : 1ull;
     };
-    // A logit into the first CTA's list.  Only as many as were counted ever come, and those fit; but a streamed row is read again
-    // for every pass, and no store may depend on its being what it was.
+    // A logit into the first CTA's list.  Only as many as were counted come, and those fit; but a streamed row is read again for
+    // every pass, and no store may depend on its being what it was.
+    auto listed = [&]() { return RES ? s.n_list : min(s.n_list, SV_FEW); };
     auto put = [&](float x, uint32_t i) {
-        if (const uint32_t at = atomicAdd(cl.map_shared_rank(&s.n_list, 0), 1u); at < SV_FEW) *cl.map_shared_rank(&s.list[at], 0) = sv_key(x, base + i);
+        if (const uint32_t at = atomicAdd(cl.map_shared_rank(&s.n_list, 0), 1u); RES || at < SV_FEW) *cl.map_shared_rank(&s.list[at], 0) = sv_key(x, base + i);
     };
     // The logits for which `take` says so, sorted.
     auto collect = [&](auto take) {
         each([&](float x, uint32_t i) { if (take(x, i)) put(x, i); });
         together();
-        if (rank == 0) sv_sort(s.list, min(s.n_list, SV_FEW));
+        if (rank == 0) sv_sort(s.list, listed());
     };
     constexpr int PER = SV_FEW / SV_T;                      // candidates of a thread
     // All candidates in the list: cut by the whole rule and drawn from there.  top_p is a share of `all`, or of the first
     // top_k (all = 0).
     auto few = [&](uint64_t all) {
-        const uint32_t m = min(s.n_list, SV_FEW), cand = rule.top_k > 0 ? min(m, rule.top_k) : m;
+        const uint32_t m = listed(), cand = rule.top_k > 0 ? min(m, rule.top_k) : m;
         uint64_t w[PER], mine = 0, sum;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
