@@ -164,12 +164,12 @@ static int create(const adam_b200_kv_desc& desc, uint32_t id) {
 
 bool capturing();
 // By adam_b200_capture_begin, or by the owner of a stream that the library was lent: the books would change once, the device with
-// every replay.
+// every replay.  (Nobody else captures the library's own stream, and the default stream cannot be captured.)
 static bool recording() {
-    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
     if (capturing()) return true;
-    if (cudaStreamIsCapturing(g.stream, &state) != cudaSuccess) { cudaGetLastError(); return true; }      // the default stream beside another's capture
-    return state != cudaStreamCaptureStatusNone;
+    if (g.stream == g.own_stream || g.stream == cudaStreamLegacy) return false;
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(g.stream, &state) != cudaSuccess || state != cudaStreamCaptureStatusNone;
 }
 static int page_op(uint32_t id, const char* name, KvCache** kv) {
     *kv = get_kv(id);
