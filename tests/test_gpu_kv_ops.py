@@ -670,9 +670,10 @@ def special(gpu, rng, dtype, dim, group, kv_heads, page, new, n, window, cap, sc
 
     spoil(q, put)
     got = attention(gpu, c, [0], [0, new], new, kv_heads * group, q, layer=0, window=window, cap=cap, scale=scale)
+    rows = sorted({*range(0, new, 13), *range(min(54, new), min(66, new)), new // 2, *range(max(new - 8, 0), new)})       # (54 ..: a tile's end)
     with np.errstate(all="ignore"):
-        want = np.stack([ko.attend(q[r], c.held[0][:, 0, 0], c.held[0][:, 0, 1], n - new + r, window, 0, scale, cap)[0] for r in range(min(new, 150))])
-    got, fine = got[:len(want)], np.isfinite(want)
+        want = np.stack([ko.attend(q[r], c.held[0][:, 0, 0], c.held[0][:, 0, 1], n - new + r, window, 0, scale, cap)[0] for r in rows])
+    got, fine = got[rows], np.isfinite(want)
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)].astype(np.float32))
     assert (np.abs(got[fine] - want[fine]) <= 16 * 8 * U * (1 + 50) * np.maximum(1, np.abs(want[fine]))).all()
     assert gpu.device_error() == 0
@@ -706,6 +707,17 @@ def test_attention_special_queries_and_keys(gpu, dtype, dim, group, kv_heads, pa
 def test_attention_scale_of_zero(gpu, dtype, dim, group, kv_heads, page, new, n, cap):
     """The mean of what a row sees; rows that see nothing of a chunk of positions among others that do (the first of several, too)."""
     special(gpu, np.random.default_rng(new + dim), dtype, dim, group, kv_heads, page, new, n, 7 * n // 15, cap, 0.0, lambda q, put: None)
+
+
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("dtype,dim,group,kv_heads,page,new,n", SPECIAL)
+def test_attention_negative_scale(gpu, dtype, dim, group, kv_heads, page, new, n, cap):
+    """Scores with the other sign, and a query of zeros."""
+    def spoil(q, put):
+        q[new - 1, 0] = 0.0
+        put(n - new, 0, 0, 1, 30000.0)                            # a key that decides
+
+    special(gpu, np.random.default_rng(new + dim), dtype, dim, group, kv_heads, page, new, n, 0, cap, -1e-4, spoil)
 
 
 @pytest.mark.parametrize("cap", [0.0, 50.0])
