@@ -16,7 +16,7 @@
 // SMs refill together: with loops unrolled freely it took 2600 cycles a chunk on some SMs and 4000 on others, with short ones (and
 // two values to an instruction) 2900 everywhere.  The products need 2048 of those at the tensor core's rate, shared memory 2000 for
 // what it hands to them and takes in, and an output waits for the one before it to be taken.  2048 tokens behind 14000, 32
-// heads over 16 of 128: 922 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
+// heads over 16 of 128: 925 us, two products where fp16 operands would have one, so 1.1 PFLOP/s of them.
 #include "attn_kv.cuh"
 #include "gemv_mma.cuh"
 

@@ -308,8 +308,9 @@ int adam_b200_map_ptr(uint32_t map, uint64_t* ptr_out, uint64_t* bytes_out);
  * A pool of n_pages pages of page_size positions (keys and values of every layer), and max_seqs sequences that each hold up
  * to max_pages of them.  A sequence is a number below max_seqs and has a length, 0 at first.  Which sequence holds which page
  * is host arithmetic; what follows from it on the device is enqueued like an operator, with no wait.  Pages cannot change
- * hands while a graph is being captured; a captured operator reads the lengths and pages of the time it is replayed, and must
- * not be replayed once its cache is destroyed.  No counterpart in the reference (one contiguous cache per engine,
+ * hands while a graph is being captured, be it by the owner of a lent stream; a captured operator reads the lengths and pages of
+ * the time it is replayed, must not be replayed once its cache is destroyed, nor run beside another call on the same cache
+ * (they share its workspace).  No counterpart in the reference (one contiguous cache per engine,
  * adam/models/engine.py:3045-3302). */
 typedef struct adam_b200_kv_desc {
     uint32_t n_layer, n_head_kv;
