@@ -169,7 +169,8 @@ static bool recording() {
     if (capturing()) return true;
     if (g.stream == g.own_stream || g.stream == cudaStreamLegacy) return false;
     cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
-    return cudaStreamIsCapturing(g.stream, &state) != cudaSuccess || state != cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(g.stream, &state) != cudaSuccess) { cudaGetLastError(); return true; }
+    return state != cudaStreamCaptureStatusNone;
 }
 static int page_op(uint32_t id, const char* name, KvCache** kv) {
     *kv = get_kv(id);
