@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(SV_T, 1) k_sample_vocab(const SampleArgs a) {
             const uint64_t k = sv_key(x, base + i);
             return k >= lo && k <= hi;
         };
-        while (in > SV_FEW) {
+        for (int turn = 0; in > SV_FEW && turn < 6; ++turn) {          // (11 of 64 bits each; a row that is written meanwhile may stay above)
             if (!ranged) {
                 uint64_t k0 = ~0ull, k1 = 0;
                 each([&](float x, uint32_t i) { if (inside(x, i)) { const uint64_t k = sv_key(x, base + i); k0 = min(k0, k); k1 = max(k1, k); } });
